@@ -18,6 +18,7 @@ from .api import (gemm_fp16, gemm_fp16_batched, gemm_int8, gemm_int8_rowcol, gem
                   flash_attention,
                   set_dispatch_override, set_weight_prefetch,
                   describe_dispatch, device_error, version)
+from .paged import (PagedCache, rope_table, qk_norm_rope, paged_attention, evict_cache)  # noqa: F401
 from .nsplit import NSplit, col_begin  # noqa: F401
 
 __all__ = [
@@ -25,6 +26,7 @@ __all__ = [
     "debug_int8_acc", "debug_int4_group_acc", "debug_stream_read", "debug_stream_k_plan",
     "debug_peer_wait_timeout", "debug_exp2_poly", "quantize_int4",
     "swiglu_fused", "flash_attention",
+    "PagedCache", "rope_table", "qk_norm_rope", "paged_attention", "evict_cache",
     "set_dispatch_override",
     "set_weight_prefetch",
     "describe_dispatch",

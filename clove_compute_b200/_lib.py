@@ -22,6 +22,16 @@ _I = ctypes.c_int
 _F = ctypes.c_float
 _I8 = ctypes.c_int8
 _SZ = ctypes.c_size_t
+_LL = ctypes.c_longlong
+
+
+class PagedCacheStruct(ctypes.Structure):
+    """clove_paged_cache of include/clove/capi.h."""
+    _fields_ = [("K", _P), ("V", _P), ("num_pages", _I), ("page_size", _I), ("num_kv_heads", _I),
+                ("head_dim", _I), ("page_stride", _LL), ("token_stride", _LL), ("head_stride", _LL),
+                ("dtype", _I), ("k_scale", _F), ("v_scale", _F)]
+
+
 
 # name -> (argtypes, restype); mirrors include/clove/capi.h.
 SIGNATURES = {
@@ -35,6 +45,11 @@ SIGNATURES = {
     "clove_gemm_int8_rowcol": ([_P, _P, _P, _I, _I, _I, _P, _P, _P], _I),
     "clove_gemm_int4": ([_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P], _I),
     "clove_flash_attention": ([_P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _I, _I, _P], _I),
+    "clove_qk_norm_rope": ([_P, _P, _P, _LL, _LL, _LL, _P, _P, _F, _P, _I, _I, _I, _P, _P, _P, _P,
+                            _LL, _P, _LL, _I, _I, _I, _I, _I, _P], _I),
+    "clove_paged_attention": ([_P, _LL, _P, _P, _LL, _I, _P, _P, _LL, _P, _P, _I, _I, _I, _F, _I, _I,
+                               _P], _I),
+    "clove_evict_cache": ([_P, _P, _P, _LL, _I, _P, _P, _LL, _I, _P, _P, _I, _I, _I, _P], _I),
     "clove_debug_int8_acc": ([_P, _P, _P, _I, _I, _I, _I8, _I8, _P], _I),
     "clove_debug_int4_group_acc": ([_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P], _I),
     "clove_quantize_int4": ([_P, _I, _I, _P, _P, _P, _P], _I),

@@ -1,0 +1,672 @@
+// paged_attention_sm100.cuh -- attention of one new token per sequence over a paged
+// key-value cache (decode), split over the cache's length and joined.
+//
+//   s_t = scale * q . k_t,   O = sum_t exp(s_t) v_t / sum_t exp(s_t),
+//   LSE = log sum_t exp(s_t)   over the sequence's keys t (the last `window` of them)
+//
+// Each K and V element is used by the query heads of one group only (1 to 16 products per
+// element), so the kernel is bound by reading the cache once, and everything serves that:
+//
+// * Work split. An item is one (sequence, key head, block of up to 8 or 16 of its query
+//   heads); its keys are cut into tiles of 64. All tiles of all items, in order, are dealt
+//   out evenly: CTA c of W takes tiles [c N / W, (c+1) N / W). So ragged batches, a single
+//   long sequence and many short ones all load every SM alike, with at most two unfinished
+//   items per CTA. Those are left as partial sums in a workspace and joined by a second,
+//   programmatically overlapped kernel in a fixed order (results do not depend on timing;
+//   no counters to keep zeroed between calls, nothing that two captured graphs could
+//   share). Lengths are read on the device: one captured launch serves every step.
+// * Loads. Four warps per CTA, each with its own ring of 16-key K and V chunks filled by
+//   16-byte cp.async (any page size, order and strides), no CTA barrier until an item
+//   ends. Two CTAs per SM keep about 128 KB in flight per SM. The ring runs across items.
+// * Products. S^T = K Q^T and O^T = V^T P^T as m16n8k16 matrix instructions with the keys
+//   (or head elements) as the 16 rows and 8 query heads as the columns: a group of up to 8
+//   heads wastes nothing that costs time. (tcgen05 wants 64 or 128 rows of queries.)
+//   K and V reach the instructions by ldmatrix from XOR-swizzled rows; e4m3 elements are
+//   widened in registers. P is passed as the sum of two 16-bit halves, so that no weight
+//   is rounded; scores, maxima, totals and O stay in fp32.
+// * Softmax. Running maximum and total per warp; the maximum is reduced over the warp
+//   only when some lane's score exceeds it.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include "paged_cache.cuh"
+
+namespace clove {
+namespace kern {
+
+constexpr int kPagedWarps = kPagedTile / 16;
+
+template <bool F8, int D, int NT>
+struct PagedShape {
+  static constexpr int THREADS = kPagedWarps * 32;
+  static constexpr int HEADS = 8 * NT;             // query heads per item
+  static constexpr int ROWB = D * (F8 ? 1 : 2);    // bytes of a K (or V) row
+  static constexpr int CPR = ROWB / 16;            // 16-byte pieces per row
+  static constexpr int CHUNK = 16 * ROWB;          // bytes of a warp's K (or V) chunk
+  // 24 KB of ring per warp where that holds three chunks (two CTAs per SM), else three
+  // chunks (head_dim 256 in 16 bits: one CTA per SM).
+  static constexpr int STAGES = 24576 / (2 * CHUNK) >= 8 ? 8
+                                : 24576 / (2 * CHUNK) >= 3 ? 24576 / (2 * CHUNK) : 3;
+  static constexpr int RING = STAGES * 2 * CHUNK;  // per warp
+  static constexpr int OPITCH = D + 4;             // floats; conflict-free column writes
+  static constexpr int MERGE = kPagedWarps * 8 * OPITCH * 4;
+  static constexpr int SMEM = kPagedWarps * RING + MERGE + kPagedWarps * HEADS * 2 * 4;
+  static constexpr int CTAS_PER_SM = 2 * (SMEM + 1024) <= 228 * 1024 ? 2 : 1;
+};
+
+// ---- 16-bit types: pairs, conversion, the matrix instruction
+template <typename T>
+struct Pair;
+template <>
+struct Pair<__half> {
+  __device__ static __forceinline__ uint32_t pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  __device__ static __forceinline__ float2 unpack(uint32_t v) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&v));
+  }
+  __device__ static __forceinline__ uint32_t from_e4m3(uint16_t v) {
+    const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2(v, __NV_E4M3);
+    return static_cast<uint32_t>(r.x) | (static_cast<uint32_t>(r.y) << 16);
+  }
+  __device__ static __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                             uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+};
+template <>
+struct Pair<__nv_bfloat16> {
+  __device__ static __forceinline__ uint32_t pack(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  __device__ static __forceinline__ float2 unpack(uint32_t v) {
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+  }
+  // Exact: every e4m3 value is a bf16 value.
+  __device__ static __forceinline__ uint32_t from_e4m3(uint16_t v) {
+    const float2 f = Pair<__half>::unpack(Pair<__half>::from_e4m3(v));
+    return pack(f.x, f.y);
+  }
+  __device__ static __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                             uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+};
+
+__device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+// 16 bytes global -> shared; src_bytes 0 fills zeros and reads nothing.
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, uint32_t src_bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(src_bytes)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Place of a CTA in the tile order: item, its sequence and the tile within it.
+struct PagedCursor {
+  int b;     // sequence
+  int hh;    // (key head, head block) within the sequence
+  int tile;  // tile within the item
+  PagedSpan s;
+};
+__device__ __forceinline__ void paged_next_item(const PagedAttnParams& p, PagedCursor& c, int hh_n) {
+  c.tile = 0;
+  if (++c.hh < hh_n) return;
+  c.hh = 0;
+  do {
+    ++c.b;
+    if (c.b >= p.batch) {
+      c.s = PagedSpan{0, 0, 0, 0};
+      return;
+    }
+    c.s = paged_span(p, c.b);
+  } while (c.s.tiles == 0);
+}
+
+// The total number of tiles, and (warp-uniform) the cursor of tile `begin(total)` for this
+// CTA. Lane l sums the sequences [l R, (l+1) R); the lane that holds the tile is found by
+// a scan and its sequences are scanned again in strips of 32.
+__device__ __forceinline__ long long paged_total(const PagedAttnParams& p, int hh_n, int per_lane,
+                                                 long long* lane_sum) {
+  const int lane = static_cast<int>(dev::lane_idx());
+  long long sum = 0;
+  const int b0 = lane * per_lane, b1 = min(p.batch, b0 + per_lane);
+  for (int b = b0; b < b1; ++b) sum += paged_span(p, b).tiles;
+  sum *= hh_n;
+  *lane_sum = sum;
+  long long total = sum;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  return total;
+}
+__device__ __forceinline__ PagedCursor paged_find(const PagedAttnParams& p, int hh_n, int per_lane,
+                                                  long long lane_sum, long long at) {
+  const int lane = static_cast<int>(dev::lane_idx());
+  long long pre = lane_sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, pre, o);
+    if (lane >= o) pre += v;
+  }
+  // First lane whose inclusive prefix exceeds `at`.
+  const unsigned above = __ballot_sync(0xffffffffu, pre > at);
+  const int owner = above ? __ffs(above) - 1 : 31;
+  long long before = __shfl_sync(0xffffffffu, pre - lane_sum, owner);
+  PagedCursor c{p.batch, 0, 0, {0, 0, 0, 0}};
+  const int b_end = min(p.batch, (owner + 1) * per_lane);
+  for (int b0 = owner * per_lane; b0 < b_end; b0 += 32) {
+    const int b = b0 + lane;
+    const long long t = b < b_end ? static_cast<long long>(paged_span(p, b).tiles) * hh_n : 0;
+    long long inc = t;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, before + inc > at);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      const long long start = before + __shfl_sync(0xffffffffu, inc - t, l);
+      c.b = b0 + l;
+      c.s = paged_span(p, c.b);
+      const long long in = at - start;
+      c.hh = static_cast<int>(in / c.s.tiles);
+      c.tile = static_cast<int>(in - static_cast<long long>(c.hh) * c.s.tiles);
+      return c;
+    }
+    before += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  return c;
+}
+
+template <typename T, bool F8, int D, int NT>
+__global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
+                                  PagedShape<F8, D, NT>::CTAS_PER_SM)
+    paged_attention_kernel(const PagedAttnParams p) {
+  using S = PagedShape<F8, D, NT>;
+  using P2 = Pair<T>;
+  constexpr int ROWB = S::ROWB, CPR = S::CPR, KK = D / 16;
+  extern __shared__ __align__(128) uint8_t smem[];
+  float* merge = reinterpret_cast<float*>(smem + kPagedWarps * S::RING);
+  float* sm_m = merge + S::MERGE / 4;         // [warp][HEADS]
+  float* sm_l = sm_m + kPagedWarps * S::HEADS;
+  const int lane = static_cast<int>(dev::lane_idx());
+  const int warp = static_cast<int>(dev::warp_idx());
+  const int cta = static_cast<int>(blockIdx.x);
+  const uint32_t ring = dev::smem_u32(smem) + warp * S::RING;
+  const int hh_n = p.cache.kv_heads * p.blocks;
+  const int row4 = lane >> 2, col4 = lane & 3;
+
+  dev::grid_dependency_wait();
+  dev::allow_dependent_launch();
+
+  // Sequences without keys: zeros. Bad lengths are clamped and reported.
+  for (int b = cta; b < p.batch; b += static_cast<int>(gridDim.x)) {
+    const int n = p.seq_lens[b];
+    if ((n < 0 || n > p.capacity) && threadIdx.x == 0) dev::record_error(dev::kDevErrBadIndex);
+    if (n > 0) continue;
+    T* o = static_cast<T*>(p.o) + b * p.o_stride;
+    for (int i = static_cast<int>(threadIdx.x) * 8; i < p.heads * D; i += S::THREADS * 8)
+      *reinterpret_cast<uint4*>(o + i) = make_uint4(0u, 0u, 0u, 0u);
+    if (p.lse != nullptr)
+      for (int i = static_cast<int>(threadIdx.x); i < p.heads; i += S::THREADS)
+        p.lse[static_cast<long long>(b) * p.heads + i] = __int_as_float(0xff800000);
+  }
+
+  const int per_lane = (p.batch + 31) / 32;
+  long long lane_sum;
+  const long long total = paged_total(p, hh_n, per_lane, &lane_sum);
+  const long long workers = min(static_cast<long long>(gridDim.x), total);
+  int* meta = p.meta + cta * kPagedMeta;
+  if (cta >= workers) {
+    if (threadIdx.x == 0) meta[0] = -1, meta[2] = -1;
+    return;
+  }
+  const long long t_begin = cta * total / workers, t_end = (cta + 1) * total / workers;
+  const int n_tiles = static_cast<int>(t_end - t_begin);
+  PagedCursor cur = paged_find(p, hh_n, per_lane, lane_sum, t_begin);
+  PagedCursor ld = cur;  // the loads' place
+  int ld_left = n_tiles;
+  const int page_mask = (1 << p.cache.page_shift) - 1;
+  const bool whole_pages = p.cache.page_shift >= 4;  // a 16-key chunk lies in one page
+
+  // Page of the chunk that is loaded next, read one step ahead of its use.
+  auto chunk_key = [&](const PagedCursor& c) { return c.s.base + c.tile * kPagedTile + warp * 16; };
+  auto page_of = [&](int b, int key) {
+    const int pg = p.page_table[b * p.table_stride + (key >> p.cache.page_shift)];
+    if (pg >= 0 && pg < p.cache.num_pages) return pg;
+    dev::record_error(dev::kDevErrBadIndex);
+    return -1;
+  };
+  int ld_page = 0;
+  auto fetch_page = [&]() {
+    const int key = chunk_key(ld);
+    if (whole_pages && ld_left > 0 && key < ld.s.len) ld_page = page_of(ld.b, key);
+  };
+  auto issue = [&](int stage) {
+    if (ld_left > 0) {
+      const int key = chunk_key(ld);
+      if (key < ld.s.len) {
+        const uint32_t kdst = ring + stage * 2 * S::CHUNK, vdst = kdst + S::CHUNK;
+        const int piece = lane % CPR;
+        const long long head_off = (ld.hh / p.blocks) * p.cache.head_stride;
+        const uint8_t* kb = static_cast<const uint8_t*>(p.cache.K);
+        const uint8_t* vb = static_cast<const uint8_t*>(p.cache.V);
+        constexpr int EB = F8 ? 1 : 2;
+        const bool full = key >= ld.s.first && key + 16 <= ld.s.len;
+#pragma unroll
+        for (int r0 = 0; r0 < 16; r0 += 32 / CPR) {
+          const int r = r0 + lane / CPR;
+          const int t = key + r;
+          bool ok = full || (t >= ld.s.first && t < ld.s.len);
+          int pg = ld_page;
+          if (!whole_pages && ok) pg = page_of(ld.b, t);
+          ok = ok && pg >= 0;
+          long long off = 0;
+          if (ok)
+            off = (pg * p.cache.page_stride + (t & page_mask) * p.cache.token_stride + head_off) * EB +
+                  piece * 16;
+          const uint32_t sw = CPR >= 8 ? (piece ^ (r & 7)) : (piece ^ ((r >> 1) & 3));
+          const uint32_t d = r * ROWB + sw * 16;
+          cp_async_16(kdst + d, kb + off, ok ? 16u : 0u);
+          cp_async_16(vdst + d, vb + off, ok ? 16u : 0u);
+        }
+      }
+      --ld_left;
+      if (++ld.tile >= ld.s.tiles) paged_next_item(p, ld, hh_n);
+      fetch_page();
+    }
+    cp_async_commit();
+  };
+  fetch_page();
+#pragma unroll
+  for (int i = 0; i < S::STAGES - 1; ++i) issue(i);
+
+  uint32_t qf[NT][KK][2];
+  float o[NT][KK][4], m[NT][2], l[NT][2];
+  int stage = 0;
+  bool fresh = true;
+  int seg_begin = cur.tile;  // first tile of the current item in this CTA
+  int cont_item = -1, cont_ends = 0, open_item = -1;
+  for (int i = 0; i < n_tiles; ++i) {
+    const int h = cur.hh / p.blocks;
+    const int g0 = (cur.hh - h * p.blocks) * S::HEADS;  // first head of the block in its group
+    const int live_heads = min(S::HEADS, p.group - g0);
+    const int head0 = h * p.group + g0;
+    if (fresh) {
+      fresh = false;
+      seg_begin = cur.tile;
+      const T* q = static_cast<const T*>(p.q) + cur.b * p.q_stride + static_cast<long long>(head0) * D;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int n = nt * 8 + row4;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+          qf[nt][kk][0] = qf[nt][kk][1] = 0u;
+          if (n < live_heads) {
+            // The k order within 16 elements follows the K fragments: see below.
+            const T* x = q + static_cast<long long>(n) * D + kk * 16 + (F8 ? 4 : 2) * col4;
+            qf[nt][kk][0] = *reinterpret_cast<const uint32_t*>(x);
+            qf[nt][kk][1] = *reinterpret_cast<const uint32_t*>(x + (F8 ? 2 : 8));
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[nt][kk][e] = 0.f;
+        }
+        m[nt][0] = m[nt][1] = __int_as_float(0xff800000);
+        l[nt][0] = l[nt][1] = 0.f;
+      }
+    }
+    cp_async_wait<S::STAGES - 2>();
+    __syncwarp();
+    issue(stage == 0 ? S::STAGES - 1 : stage - 1);
+
+    const int key = chunk_key(cur);
+    if (key < cur.s.len) {
+      const uint32_t ks = ring + stage * 2 * S::CHUNK, vs = ks + S::CHUNK;
+      float sc[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[nt][e] = 0.f;
+      // S^T: rows = keys, columns = heads. ldmatrix lane addresses: lanes 0-15 name rows
+      // 0-15 of the left 16 bytes, lanes 16-31 of the right 16 bytes.
+      {
+        const int r = lane & 15;
+        const uint32_t row = ks + r * ROWB;
+        const int sw = CPR >= 8 ? (r & 7) : ((r >> 1) & 3);
+#pragma unroll
+        for (int c = 0; c < CPR; c += 2) {
+          uint32_t a[4];
+          ldsm_x4(a, row + (((c + (lane >> 4)) ^ sw) << 4));
+          if (!F8) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) P2::mma(sc[nt], a, qf[nt][c / 2][0], qf[nt][c / 2][1]);
+          } else {
+            // A lane holds four consecutive elements of a row: the first two stand in for
+            // k = 2c, 2c+1 and the others for k = 2c+8, 2c+9, in Q's fragments alike.
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              uint32_t x[4];
+              x[0] = P2::from_e4m3(static_cast<uint16_t>(a[2 * w]));
+              x[1] = P2::from_e4m3(static_cast<uint16_t>(a[2 * w + 1]));
+              x[2] = P2::from_e4m3(static_cast<uint16_t>(a[2 * w] >> 16));
+              x[3] = P2::from_e4m3(static_cast<uint16_t>(a[2 * w + 1] >> 16));
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) P2::mma(sc[nt], x, qf[nt][c + w][0], qf[nt][c + w][1]);
+            }
+          }
+        }
+      }
+      const int t0 = key + row4, t1 = t0 + 8;
+      const bool full = key >= cur.s.first && key + 16 <= cur.s.len;
+      const bool ok0 = full || (t0 >= cur.s.first && t0 < cur.s.len);
+      const bool ok1 = full || (t1 >= cur.s.first && t1 < cur.s.len);
+      bool up = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          sc[nt][e] *= p.scale_log2;
+          if (!(e < 2 ? ok0 : ok1)) sc[nt][e] = __int_as_float(0xff800000);
+        }
+        up = up || fmaxf(sc[nt][0], sc[nt][2]) > m[nt][0] || fmaxf(sc[nt][1], sc[nt][3]) > m[nt][1];
+      }
+      if (p.scores != nullptr) {
+        float* out = p.scores +
+                     ((static_cast<long long>(cur.b) * p.cache.kv_heads + h) * p.capacity) * p.group + g0;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int n = nt * 8 + col4 * 2 + (e & 1);
+            if (n < live_heads && (e < 2 ? ok0 : ok1))
+              out[static_cast<long long>(e < 2 ? t0 : t1) * p.group + n] = sc[nt][e];
+          }
+      }
+      if (__any_sync(0xffffffffu, up)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float v = fmaxf(m[nt][e], fmaxf(sc[nt][e], sc[nt][e + 2]));
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, x));
+            // All scores -inf so far: nothing to rescale.
+            const float alpha = v == m[nt][e] ? 1.f : dev::ex2_approx(m[nt][e] - v);
+            m[nt][e] = v;
+            l[nt][e] *= alpha;
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) {
+              o[nt][kk][e] *= alpha;
+              o[nt][kk][e + 2] *= alpha;
+            }
+          }
+      }
+      // P^T as the B operand: transposed 8 x 8 blocks of the score fragments; two 16-bit
+      // halves whose sum is p to fp32's precision (fp16: to 2^-25 of the largest weight).
+      uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float mm0 = m[nt][0] == __int_as_float(0xff800000) ? 0.f : m[nt][0];
+          const float mm1 = m[nt][1] == __int_as_float(0xff800000) ? 0.f : m[nt][1];
+          const float p0 = dev::ex2_approx(sc[nt][2 * e] - mm0);
+          const float p1 = dev::ex2_approx(sc[nt][2 * e + 1] - mm1);
+          l[nt][0] += p0;
+          l[nt][1] += p1;
+          const uint32_t hi = P2::pack(p0, p1);
+          const float2 f = P2::unpack(hi);
+          ph[nt][e] = transpose_8x8(hi);
+          pl[nt][e] = transpose_8x8(P2::pack(p0 - f.x, p1 - f.y));
+        }
+      }
+      // O^T += V^T P^T: rows = head elements. 16-bit: tile kk holds elements 16 kk + row.
+      // e4m3: ldmatrix moves pairs of elements; tile row j < 8 is element 16 kk + 2 j, row
+      // 8 + j element 16 kk + 2 j + 1.
+      if (!F8) {
+        const int r = (lane & 7) + ((lane >> 4) << 3);
+        const uint32_t row = vs + r * ROWB;
+        const int sw = r & 7;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+          uint32_t a[4];
+          ldsm_x4_t(a, row + (((2 * kk + ((lane >> 3) & 1)) ^ sw) << 4));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            P2::mma(o[nt][kk], a, ph[nt][0], ph[nt][1]);
+            P2::mma(o[nt][kk], a, pl[nt][0], pl[nt][1]);
+          }
+        }
+      } else {
+        const int r = lane & 15;
+        const uint32_t row = vs + r * ROWB;
+        const int sw = CPR >= 8 ? (r & 7) : ((r >> 1) & 3);
+#pragma unroll
+        for (int k2 = 0; k2 < KK; k2 += 2) {
+          uint32_t a[4];
+          ldsm_x4_t(a, row + (((k2 + (lane >> 4)) ^ sw) << 4));
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const uint32_t lo = __byte_perm(a[2 * w], 0u, 0x3120);
+            const uint32_t hi = __byte_perm(a[2 * w + 1], 0u, 0x3120);
+            uint32_t x[4];
+            x[0] = P2::from_e4m3(static_cast<uint16_t>(lo));
+            x[1] = P2::from_e4m3(static_cast<uint16_t>(lo >> 16));
+            x[2] = P2::from_e4m3(static_cast<uint16_t>(hi));
+            x[3] = P2::from_e4m3(static_cast<uint16_t>(hi >> 16));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              P2::mma(o[nt][k2 + w], x, ph[nt][0], ph[nt][1]);
+              P2::mma(o[nt][k2 + w], x, pl[nt][0], pl[nt][1]);
+            }
+          }
+        }
+      }
+    }
+    stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+
+    const bool item_ends = cur.tile + 1 == cur.s.tiles;
+    if (item_ends || i + 1 == n_tiles) {
+      // Join the four warps; write the result, or a partial one where the item goes on in
+      // (or came from) another CTA.
+      const bool begins = seg_begin == 0;
+      const bool whole = begins && item_ends;
+      const int item = cur.b * hh_n + cur.hh;
+      const int slot = 2 * cta + (begins ? 1 : 0);
+      if (!whole) {
+        if (begins) open_item = item;
+        else cont_item = item, cont_ends = item_ends ? 1 : 0;
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float v = l[nt][e];
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) v += __shfl_xor_sync(0xffffffffu, v, x);
+          if (row4 == 0) {
+            sm_m[warp * S::HEADS + nt * 8 + col4 * 2 + e] = m[nt][e];
+            sm_l[warp * S::HEADS + nt * 8 + col4 * 2 + e] = v;
+          }
+        }
+      __syncthreads();
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float* mine = merge + warp * 8 * S::OPITCH;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int n = nt * 8 + col4 * 2 + e;
+          float top = sm_m[n];
+#pragma unroll
+          for (int w = 1; w < kPagedWarps; ++w) top = fmaxf(top, sm_m[w * S::HEADS + n]);
+          const float f = m[nt][e] == top ? 1.f : dev::ex2_approx(m[nt][e] - top);
+#pragma unroll
+          for (int kk = 0; kk < KK; ++kk) {
+            const int d0 = kk * 16 + (F8 ? 2 * row4 : row4), d1 = d0 + (F8 ? 1 : 8);
+            mine[(col4 * 2 + e) * S::OPITCH + d0] = o[nt][kk][e] * f;
+            mine[(col4 * 2 + e) * S::OPITCH + d1] = o[nt][kk][e + 2] * f;
+          }
+        }
+        __syncthreads();
+        for (int idx = static_cast<int>(threadIdx.x); idx < 8 * (D / 4); idx += S::THREADS) {
+          const int j = idx / (D / 4), d = (idx - j * (D / 4)) * 4, n = nt * 8 + j;
+          if (n >= live_heads) continue;
+          float top = sm_m[n];
+#pragma unroll
+          for (int w = 1; w < kPagedWarps; ++w) top = fmaxf(top, sm_m[w * S::HEADS + n]);
+          float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int w = 0; w < kPagedWarps; ++w) {
+            const float mw = sm_m[w * S::HEADS + n];
+            sum += sm_l[w * S::HEADS + n] * (mw == top ? 1.f : dev::ex2_approx(mw - top));
+            const float4 x = *reinterpret_cast<const float4*>(merge + (w * 8 + j) * S::OPITCH + d);
+            v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
+          }
+          if (whole) {
+            const float inv = p.v_scale / sum;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] *= inv;
+            T* out = static_cast<T*>(p.o) + cur.b * p.o_stride + static_cast<long long>(head0 + n) * D + d;
+            *reinterpret_cast<uint2*>(out) = Quad<T>::pack(v);
+            if (d == 0) {
+              const float l2 = top + log2f(sum);
+              const long long at = static_cast<long long>(cur.b) * p.heads + head0 + n;
+              if (p.lse != nullptr) p.lse[at] = l2 * 0.6931471805599453f;
+              if (p.lse2 != nullptr) p.lse2[at] = l2;
+            }
+          } else {
+            const long long at = static_cast<long long>(slot) * S::HEADS + n;
+            *reinterpret_cast<float4*>(p.part_o + at * D + d) = make_float4(v[0], v[1], v[2], v[3]);
+            if (d == 0) {
+              p.part_m[at] = top;
+              p.part_l[at] = sum;
+            }
+          }
+        }
+        __syncthreads();
+      }
+      fresh = true;
+    }
+    if (item_ends) paged_next_item(p, cur, hh_n);
+    else ++cur.tile;
+  }
+  cp_async_wait<0>();
+  if (threadIdx.x == 0) {
+    meta[0] = cont_item;
+    meta[1] = cont_ends;
+    meta[2] = open_item;
+  }
+}
+
+// Joins the items that more than one CTA worked on: block c takes the item that CTA c
+// opened and did not finish (if any). Its parts are CTA c's second partial and the first
+// partials of the CTAs behind it, up to the one that ends the item. One warp per head, the
+// parts in order: O = sum_k O_k 2^(m_k - M) / sum_k l_k 2^(m_k - M).
+template <typename T, int D, int HEADS>
+__global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p) {
+  const int c = static_cast<int>(blockIdx.x);
+  dev::grid_dependency_wait();
+  const int item = p.meta[c * kPagedMeta + 2];
+  if (item < 0) return;
+  const int lane = static_cast<int>(dev::lane_idx());
+  // CTA behind the last contributor: the first one whose first item is this one and ends.
+  int last = c + 1;
+  for (;; last += 32) {
+    const int k = last + lane;
+    const bool end = k < static_cast<int>(gridDim.x) && p.meta[k * kPagedMeta + 1] != 0 &&
+                     p.meta[k * kPagedMeta] == item;
+    const unsigned hit = __ballot_sync(0xffffffffu, end);
+    if (hit) {
+      last += __ffs(hit) - 1;
+      break;
+    }
+    if (last + 32 >= static_cast<int>(gridDim.x)) return;  // not reached: every open item ends
+  }
+  const int hh_n = p.cache.kv_heads * p.blocks;
+  const int b = item / hh_n, hh = item - b * hh_n, h = hh / p.blocks;
+  const int g0 = (hh - h * p.blocks) * HEADS;
+  const int live_heads = min(HEADS, p.group - g0);
+  const int parts = last - c + 1;
+  for (int n = static_cast<int>(dev::warp_idx()); n < live_heads; n += 8) {
+    auto at = [&](int k) {
+      return static_cast<long long>(k == 0 ? 2 * c + 1 : 2 * (c + k)) * HEADS + n;
+    };
+    float top = __int_as_float(0xff800000);
+    for (int k = lane; k < parts; k += 32) top = fmaxf(top, p.part_m[at(k)]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    constexpr int V = D / 32;  // consecutive elements per lane: 2, 4 or 8
+    float acc[V], sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] = 0.f;
+    for (int k0 = 0; k0 < parts; k0 += 32) {
+      float f = 0.f, fl = 0.f;
+      if (k0 + lane < parts) {
+        const float mk = p.part_m[at(k0 + lane)];
+        f = mk == top ? 1.f : dev::ex2_approx(mk - top);
+        fl = f * p.part_l[at(k0 + lane)];
+      }
+      const int kn = min(32, parts - k0);
+#pragma unroll 4
+      for (int k = 0; k < kn; ++k) {
+        const float fk = __shfl_sync(0xffffffffu, f, k);
+        sum += __shfl_sync(0xffffffffu, fl, k);
+        const float* src = p.part_o + at(k0 + k) * D + lane * V;
+#pragma unroll
+        for (int e = 0; e < V; e += 2) {
+          const float2 x = *reinterpret_cast<const float2*>(src + e);
+          acc[e] += fk * x.x;
+          acc[e + 1] += fk * x.y;
+        }
+      }
+    }
+    const float inv = p.v_scale / sum;
+    T* out = static_cast<T*>(p.o) + b * p.o_stride + static_cast<long long>(h * p.group + g0 + n) * D +
+             lane * V;
+#pragma unroll
+    for (int e = 0; e < V; e += 2)
+      *reinterpret_cast<uint32_t*>(out + e) = Pair<T>::pack(acc[e] * inv, acc[e + 1] * inv);
+    if (lane == 0) {
+      const float l2 = top + log2f(sum);
+      const long long i = static_cast<long long>(b) * p.heads + h * p.group + g0 + n;
+      if (p.lse != nullptr) p.lse[i] = l2 * 0.6931471805599453f;
+      if (p.lse2 != nullptr) p.lse2[i] = l2;
+    }
+  }
+}
+
+}  // namespace kern
+}  // namespace clove

@@ -21,6 +21,7 @@ enum DeviceError : int {
   kDevErrNone = 0,
   kDevErrWaitTimeout = 1,   // an mbarrier wait ran past kWaitTimeoutNs
   kDevErrBadLaunch = 2,     // kernel launched with a shape it does not support
+  kDevErrBadIndex = 3,      // a position, slot, page or length outside its range; not followed
 };
 
 static __device__ int g_device_error = 0;

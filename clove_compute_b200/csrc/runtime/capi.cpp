@@ -188,8 +188,11 @@ int clove_get_device_error(int* code) {
   int rc = check_cuda(cudaDeviceSynchronize(), "cudaDeviceSynchronize");
   if (rc) return rc;
   int v = 0;
-  const int readers[5] = {read_clear_error_tc(), read_clear_error_gemv(), read_clear_error_simt(),
-                          read_clear_error_int4(), read_clear_error_attn()};
+  const int readers[] = {read_clear_error_tc(),   read_clear_error_gemv(),
+                         read_clear_error_simt(), read_clear_error_int4(),
+                         read_clear_error_attn(), read_clear_error_rope(),
+                         read_clear_error_paged_f16(), read_clear_error_paged_bf16(),
+                         read_clear_error_evict()};
   for (int r : readers) {
     if (r < 0) return fail(CLOVE_ERR_CUDA, "reading the device error word failed");
     if (v == 0 && r != 0) v = r;

@@ -14,6 +14,9 @@ struct EpiParams;
 struct PeerOut;
 struct GemvI8Epi;
 struct SimtEpi;
+struct RopeParams;
+struct PagedAttnParams;
+struct EvictParams;
 }  // namespace kern
 
 namespace rt {
@@ -143,6 +146,25 @@ int launch_attention(const void* Q, const void* K, const void* V, void* O, int b
 int read_clear_error_attn();
 // y[i] = 2^x[i] through the attention kernel's FMA-pipe polynomial (test hook; n even).
 int launch_exp2_poly_probe(const float* x, float* y, int n, cudaStream_t stream);
+
+// ---- paged key-value cache (kernels/qk_norm_rope.cu, paged_attention_*.cu,
+// paged_key_weights.cu, evict_cache.cu)
+// cache_dtype: the cache's (or dtype without one); fills p.chunks.
+int launch_qk_norm_rope(kern::RopeParams& p, int head_dim, int dtype, int cache_dtype,
+                        const DeviceInfo& dev, cudaStream_t stream);
+int read_clear_error_rope();
+// heads: query heads per item (8 or 16); ctas: CTAs to launch (the workspace in p has two
+// partial results for each), at most paged_attention_max_ctas.
+int paged_attention_max_ctas(int head_dim, int heads, bool e4m3, const DeviceInfo& dev);
+int launch_paged_attention_f16(kern::PagedAttnParams& p, int head_dim, int heads, bool e4m3, int ctas,
+                               const DeviceInfo& dev, cudaStream_t stream);
+int launch_paged_attention_bf16(kern::PagedAttnParams& p, int head_dim, int heads, bool e4m3, int ctas,
+                                const DeviceInfo& dev, cudaStream_t stream);
+int launch_paged_key_weights(const kern::PagedAttnParams& p, cudaStream_t stream);
+int launch_evict_cache(const kern::EvictParams& p, const DeviceInfo& dev, cudaStream_t stream);
+int read_clear_error_evict();
+int read_clear_error_paged_f16();
+int read_clear_error_paged_bf16();
 
 // ---- INT4 packing tool (kernels/quant_int4.cu)
 int launch_quantize_int4(const void* W, int rows, int K, uint8_t* codes, void* scales, void* zeros,

@@ -1,0 +1,319 @@
+// paged_api.cpp -- extern "C" entry points of the paged key-value cache operators
+// (include/clove/capi.h): argument checks, workspace, dispatch.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <cstdint>
+#include <mutex>
+
+#include "../kernels/paged_params.h"
+#include "internal.h"
+
+namespace clove {
+namespace rt {
+namespace {
+
+inline bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// Stream-ordered scratch that stays with the process between calls, one pool per device;
+// under stream capture an allocation of the graph's own.
+std::mutex g_pool_mu;
+cudaMemPool_t g_pool[64];
+
+int scratch_alloc(void** out, size_t bytes, int device, cudaStream_t s) {
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  int rc = check_cuda(cudaStreamIsCapturing(s, &cap), "cudaStreamIsCapturing");
+  if (rc) return rc;
+  if (cap != cudaStreamCaptureStatusNone)
+    return check_cuda(cudaMallocAsync(out, bytes, s), "cudaMallocAsync(paged attention)");
+  cudaMemPool_t pool;
+  {
+    std::lock_guard<std::mutex> lock(g_pool_mu);
+    if (g_pool[device & 63] == nullptr) {
+      cudaMemPoolProps props = {};
+      props.allocType = cudaMemAllocationTypePinned;
+      props.location.type = cudaMemLocationTypeDevice;
+      props.location.id = device;
+      rc = check_cuda(cudaMemPoolCreate(&pool, &props), "cudaMemPoolCreate(paged attention)");
+      if (rc) return rc;
+      uint64_t keep = UINT64_MAX;
+      rc = check_cuda(cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep),
+                      "cudaMemPoolSetAttribute(paged attention)");
+      if (rc) {
+        cudaMemPoolDestroy(pool);
+        return rc;
+      }
+      g_pool[device & 63] = pool;
+    }
+    pool = g_pool[device & 63];
+  }
+  return check_cuda(cudaMallocFromPoolAsync(out, bytes, pool, s), "cudaMallocFromPoolAsync(paged attention)");
+}
+
+// Checks a cache description and converts it; `dtype` is the 16-bit type it is used with.
+int take_cache(const clove_paged_cache* c, int dtype, kern::PagedCache* out) {
+  if (c == nullptr) return fail(CLOVE_ERR_INVALID_ARG, "cache is NULL");
+  if (c->K == nullptr || c->V == nullptr) return fail(CLOVE_ERR_INVALID_ARG, "cache: null K or V");
+  if (c->num_pages <= 0 || c->num_kv_heads <= 0)
+    return fail(CLOVE_ERR_INVALID_ARG, "cache: num_pages and num_kv_heads must be positive");
+  if (c->page_size <= 0 || (c->page_size & (c->page_size - 1)) != 0)
+    return fail(CLOVE_ERR_UNSUPPORTED, "cache: page_size %d is not a power of two", c->page_size);
+  if (static_cast<long long>(c->num_pages) * c->page_size > INT_MAX)
+    return fail(CLOVE_ERR_UNSUPPORTED, "cache: more than 2^31 - 1 slots");
+  if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
+    return fail(CLOVE_ERR_UNSUPPORTED, "cache: head_dim %d (64, 128 and 256 are supported)", c->head_dim);
+  if (c->dtype != CLOVE_DTYPE_F16 && c->dtype != CLOVE_DTYPE_BF16 && c->dtype != CLOVE_DTYPE_E4M3)
+    return fail(CLOVE_ERR_INVALID_ARG, "cache: unknown dtype %d", c->dtype);
+  if (dtype >= 0 && c->dtype != dtype && c->dtype != CLOVE_DTYPE_E4M3)
+    return fail(CLOVE_ERR_UNSUPPORTED, "cache: its type must be the operands' or e4m3");
+  const int eb = c->dtype == CLOVE_DTYPE_E4M3 ? 1 : 2;
+  if (!aligned(c->K, 16) || !aligned(c->V, 16) || (c->page_stride * eb) % 16 != 0 ||
+      (c->token_stride * eb) % 16 != 0 || (c->head_stride * eb) % 16 != 0)
+    return fail(CLOVE_ERR_UNSUPPORTED, "cache: K, V and the strides must be multiples of 16 bytes");
+  if (c->page_stride < 0 || c->token_stride < 0 || c->head_stride < 0)
+    return fail(CLOVE_ERR_INVALID_ARG, "cache: negative stride");
+  if (!(c->k_scale > 0.f) || !(c->v_scale > 0.f) || !std::isfinite(c->k_scale) || !std::isfinite(c->v_scale))
+    return fail(CLOVE_ERR_INVALID_ARG, "cache: scales must be positive and finite");
+  if (eb == 2 && (c->k_scale != 1.f || c->v_scale != 1.f))
+    return fail(CLOVE_ERR_INVALID_ARG, "cache: only an e4m3 cache has scales");
+  out->K = c->K;
+  out->V = c->V;
+  out->num_pages = c->num_pages;
+  out->page_shift = 0;
+  while ((1 << out->page_shift) < c->page_size) ++out->page_shift;
+  out->kv_heads = c->num_kv_heads;
+  out->page_stride = c->page_stride;
+  out->token_stride = c->token_stride;
+  out->head_stride = c->head_stride;
+  out->k_scale = c->k_scale;
+  out->v_scale = c->v_scale;
+  return CLOVE_OK;
+}
+
+}  // namespace
+}  // namespace rt
+}  // namespace clove
+
+using namespace clove;
+using namespace clove::rt;
+
+extern "C" {
+
+int clove_qk_norm_rope(const void* Q, const void* K, const void* V, long long q_stride,
+                       long long k_stride, long long v_stride, const void* q_weight,
+                       const void* k_weight, float eps, const float* rope_table, int table_len,
+                       int rotary_dim, int interleaved, const int* positions,
+                       const clove_paged_cache* cache, const int* slots, void* Q_out,
+                       long long q_out_stride, void* K_out, long long k_out_stride, int num_tokens,
+                       int num_heads, int num_kv_heads, int head_dim, int dtype, void* stream) {
+  if (num_tokens < 0) return fail(CLOVE_ERR_INVALID_ARG, "negative num_tokens");
+  if (num_heads <= 0 || num_kv_heads <= 0)
+    return fail(CLOVE_ERR_INVALID_ARG, "num_heads and num_kv_heads must be positive");
+  if (dtype != CLOVE_DTYPE_F16 && dtype != CLOVE_DTYPE_BF16)
+    return fail(CLOVE_ERR_INVALID_ARG, "dtype must be CLOVE_DTYPE_F16 or CLOVE_DTYPE_BF16");
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+    return fail(CLOVE_ERR_UNSUPPORTED, "head_dim %d (64, 128 and 256 are supported)", head_dim);
+  if (rotary_dim <= 0 || rotary_dim % 8 != 0 || rotary_dim > head_dim)
+    return fail(CLOVE_ERR_UNSUPPORTED, "rotary_dim %d must be a multiple of 8 up to head_dim", rotary_dim);
+  if (table_len <= 0) return fail(CLOVE_ERR_INVALID_ARG, "the rotation table is empty");
+  if ((q_weight == nullptr) != (k_weight == nullptr))
+    return fail(CLOVE_ERR_INVALID_ARG, "q_weight and k_weight: both or neither");
+  if (!(eps >= 0.f) || !std::isfinite(eps))
+    return fail(CLOVE_ERR_INVALID_ARG, "eps must be finite and not negative");
+  kern::RopeParams p = {};
+  int cache_dtype = dtype;
+  if (cache != nullptr) {
+    const int rc = take_cache(cache, dtype, &p.cache);
+    if (rc) return rc;
+    if (cache->num_kv_heads != num_kv_heads || cache->head_dim != head_dim)
+      return fail(CLOVE_ERR_INVALID_ARG, "the cache has %d heads of %d, K has %d of %d", cache->num_kv_heads,
+                  cache->head_dim, num_kv_heads, head_dim);
+    if (num_tokens > 0 && (V == nullptr || slots == nullptr))
+      return fail(CLOVE_ERR_INVALID_ARG, "a cache needs V and slots");
+    cache_dtype = cache->dtype;
+  } else if (V != nullptr || slots != nullptr) {
+    return fail(CLOVE_ERR_INVALID_ARG, "V and slots need a cache");
+  }
+  if (num_tokens == 0) return CLOVE_OK;
+  if (Q == nullptr || K == nullptr || Q_out == nullptr || rope_table == nullptr || positions == nullptr ||
+      (K_out == nullptr && cache == nullptr))
+    return fail(CLOVE_ERR_INVALID_ARG, "null pointer");
+  if (!aligned(Q, 16) || !aligned(K, 16) || !aligned(V, 16) || !aligned(Q_out, 16) || !aligned(K_out, 16) ||
+      !aligned(q_weight, 16) || !aligned(k_weight, 16) || !aligned(rope_table, 16))
+    return fail(CLOVE_ERR_UNSUPPORTED, "qk_norm_rope needs 16-byte aligned tensors");
+  if (!aligned(positions, 4) || !aligned(slots, 4))
+    return fail(CLOVE_ERR_INVALID_ARG, "positions and slots must be 4-byte aligned");
+  const long long qn = static_cast<long long>(num_heads) * head_dim, kn = static_cast<long long>(num_kv_heads) * head_dim;
+  if (num_tokens > 1 && (q_stride < qn || k_stride < kn || q_out_stride < qn || (K_out && k_out_stride < kn) ||
+                         (V && v_stride < kn)))
+    return fail(CLOVE_ERR_INVALID_ARG, "a token stride is smaller than the token's heads");
+  if (q_stride % 8 || k_stride % 8 || (V && v_stride % 8) || q_out_stride % 8 || (K_out && k_out_stride % 8))
+    return fail(CLOVE_ERR_UNSUPPORTED, "token strides must be multiples of 8 elements");
+  if (static_cast<long long>(num_heads) + 2LL * num_kv_heads > (1 << 24))
+    return fail(CLOVE_ERR_UNSUPPORTED, "too many heads");
+  DeviceInfo dev;
+  const int rc = current_device(&dev);
+  if (rc) return rc;
+  p.q = Q;
+  p.k = K;
+  p.v = V;
+  p.q_weight = q_weight;
+  p.k_weight = k_weight;
+  p.table = rope_table;
+  p.positions = positions;
+  p.slots = slots;
+  p.q_out = Q_out;
+  p.k_out = K_out;
+  p.q_stride = q_stride;
+  p.k_stride = k_stride;
+  p.v_stride = v_stride;
+  p.q_out_stride = q_out_stride;
+  p.k_out_stride = k_out_stride;
+  p.tokens = num_tokens;
+  p.heads = num_heads;
+  p.kv_heads = num_kv_heads;
+  p.rows = num_heads + num_kv_heads * (cache != nullptr ? 2 : 1);
+  p.table_len = table_len;
+  p.rotary = rotary_dim;
+  p.interleaved = interleaved != 0;
+  p.eps = eps;
+  return launch_qk_norm_rope(p, head_dim, dtype, cache_dtype, dev, static_cast<cudaStream_t>(stream));
+}
+
+int clove_paged_attention(const void* Q, long long q_stride, const clove_paged_cache* cache,
+                          const int* page_table, long long table_stride, int max_pages,
+                          const int* seq_lens, void* O, long long o_stride, float* lse,
+                          float* key_weights, int accumulate, int batch, int num_heads, float scale,
+                          int window, int dtype, void* stream) {
+  if (batch < 0) return fail(CLOVE_ERR_INVALID_ARG, "negative batch");
+  if (num_heads <= 0) return fail(CLOVE_ERR_INVALID_ARG, "num_heads must be positive");
+  if (dtype != CLOVE_DTYPE_F16 && dtype != CLOVE_DTYPE_BF16)
+    return fail(CLOVE_ERR_INVALID_ARG, "dtype must be CLOVE_DTYPE_F16 or CLOVE_DTYPE_BF16");
+  kern::PagedAttnParams p = {};
+  int rc = take_cache(cache, dtype, &p.cache);
+  if (rc) return rc;
+  if (num_heads % cache->num_kv_heads != 0)
+    return fail(CLOVE_ERR_INVALID_ARG, "num_heads (%d) is not a multiple of num_kv_heads (%d)", num_heads,
+                cache->num_kv_heads);
+  if (!(scale > 0.f) || !std::isfinite(scale))
+    return fail(CLOVE_ERR_INVALID_ARG, "scale must be positive and finite");
+  if (window < 0) return fail(CLOVE_ERR_INVALID_ARG, "negative window");
+  if (max_pages < 0) return fail(CLOVE_ERR_INVALID_ARG, "negative max_pages");
+  if (batch == 0) return CLOVE_OK;
+  if (Q == nullptr || O == nullptr || seq_lens == nullptr || (page_table == nullptr && max_pages > 0))
+    return fail(CLOVE_ERR_INVALID_ARG, "null pointer");
+  if (!aligned(Q, 16) || !aligned(O, 16) || q_stride % 8 || o_stride % 8)
+    return fail(CLOVE_ERR_UNSUPPORTED, "paged_attention: Q and O 16-byte aligned, strides multiples of 8 elements");
+  if (!aligned(page_table, 4) || !aligned(seq_lens, 4) || !aligned(lse, 4) || !aligned(key_weights, 4))
+    return fail(CLOVE_ERR_INVALID_ARG, "int and float arrays must be 4-byte aligned");
+  const int D = cache->head_dim;
+  if (batch > 1 && (q_stride < static_cast<long long>(num_heads) * D ||
+                    o_stride < static_cast<long long>(num_heads) * D || table_stride < max_pages))
+    return fail(CLOVE_ERR_INVALID_ARG, "a row stride is smaller than the row");
+  const long long capacity = static_cast<long long>(max_pages) * cache->page_size;
+  if (capacity > INT_MAX - 4096) return fail(CLOVE_ERR_UNSUPPORTED, "page table rows name over 2^31 tokens");
+  DeviceInfo dev;
+  rc = current_device(&dev);
+  if (rc) return rc;
+  const bool e4m3 = cache->dtype == CLOVE_DTYPE_E4M3;
+  p.q = Q;
+  p.o = O;
+  p.lse = lse;
+  p.q_stride = q_stride;
+  p.o_stride = o_stride;
+  p.page_table = page_table;
+  p.seq_lens = seq_lens;
+  p.table_stride = table_stride;
+  p.capacity = static_cast<int>(capacity);
+  p.batch = batch;
+  p.heads = num_heads;
+  p.group = num_heads / cache->num_kv_heads;
+  // Blocks of 16 heads once a group has more than 8 (one pass over the keys instead of
+  // two); head_dim 256 keeps 8, whose accumulators already take half the registers.
+  const int hb = D <= 128 && p.group > 8 ? 16 : 8;
+  p.blocks = (p.group + hb - 1) / hb;
+  p.window = window;
+  p.scale_log2 = scale * p.cache.k_scale * 1.4426950408889634f;
+  p.v_scale = p.cache.v_scale;
+  p.key_weights = key_weights;
+  p.accumulate = accumulate != 0;
+  const long long items = static_cast<long long>(batch) * p.cache.kv_heads * p.blocks;
+  if (items > INT_MAX) return fail(CLOVE_ERR_UNSUPPORTED, "paged_attention: batch x heads exceeds 2^31");
+  // As many CTAs as fit at once, or as there can be tiles. The batch's empty rows need one.
+  const long long tiles = items * ((capacity + kern::kPagedTile - 1) / kern::kPagedTile + 1);
+  const int ctas = static_cast<int>(std::min<long long>(paged_attention_max_ctas(D, hb, e4m3, dev), tiles));
+  const size_t slots = static_cast<size_t>(ctas) * 2 * hb;
+  const size_t part = slots * D * 4, stat = slots * 4, meta = static_cast<size_t>(ctas) * kern::kPagedMeta * 4;
+  const size_t heads = (static_cast<size_t>(batch) * num_heads * 4 + 255) & ~size_t(255);
+  const size_t scores = static_cast<size_t>(batch) * num_heads * static_cast<size_t>(capacity) * 4;
+  size_t bytes = part + 2 * stat + meta;
+  bytes = (bytes + 255) & ~size_t(255);
+  const size_t at_scores = bytes;
+  if (key_weights != nullptr) bytes += heads + scores;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  void* ws = nullptr;
+  rc = scratch_alloc(&ws, bytes, dev.device, s);
+  if (rc) return rc;
+  char* w = static_cast<char*>(ws);
+  p.part_o = reinterpret_cast<float*>(w);
+  p.part_m = reinterpret_cast<float*>(w + part);
+  p.part_l = reinterpret_cast<float*>(w + part + stat);
+  p.meta = reinterpret_cast<int*>(w + part + 2 * stat);
+  if (key_weights != nullptr) {
+    p.lse2 = reinterpret_cast<float*>(w + at_scores);
+    p.scores = reinterpret_cast<float*>(w + at_scores + heads);
+  }
+  rc = dtype == CLOVE_DTYPE_F16 ? launch_paged_attention_f16(p, D, hb, e4m3, ctas, dev, s)
+                                : launch_paged_attention_bf16(p, D, hb, e4m3, ctas, dev, s);
+  const int rc2 = check_cuda(cudaFreeAsync(ws, s), "cudaFreeAsync(paged attention)");
+  return rc ? rc : rc2;
+}
+
+int clove_evict_cache(const clove_paged_cache* cache, float* key_weights, const int* page_table,
+                      long long table_stride, int max_pages, const int* seq_lens, const int* dst_table,
+                      long long dst_stride, int dst_pages, int* kept, int* new_lens, int batch, int budget,
+                      int recent, void* stream) {
+  if (batch < 0) return fail(CLOVE_ERR_INVALID_ARG, "negative batch");
+  kern::EvictParams p = {};
+  int rc = take_cache(cache, -1, &p.cache);
+  if (rc) return rc;
+  if (budget <= 0) return fail(CLOVE_ERR_INVALID_ARG, "budget must be positive");
+  if (recent < 0 || recent > budget) return fail(CLOVE_ERR_INVALID_ARG, "recent must be in [0, budget]");
+  if (max_pages < 0 || dst_pages < 0) return fail(CLOVE_ERR_INVALID_ARG, "negative table width");
+  if (static_cast<long long>(dst_pages) * cache->page_size < budget)
+    return fail(CLOVE_ERR_INVALID_ARG, "dst_table rows name %lld tokens, the budget is %d",
+                static_cast<long long>(dst_pages) * cache->page_size, budget);
+  if (batch == 0) return CLOVE_OK;
+  if (key_weights == nullptr || seq_lens == nullptr || dst_table == nullptr || kept == nullptr ||
+      new_lens == nullptr || (page_table == nullptr && max_pages > 0))
+    return fail(CLOVE_ERR_INVALID_ARG, "null pointer");
+  if (!aligned(key_weights, 4) || !aligned(seq_lens, 4) || !aligned(dst_table, 4) || !aligned(kept, 4) ||
+      !aligned(new_lens, 4) || !aligned(page_table, 4))
+    return fail(CLOVE_ERR_INVALID_ARG, "int and float arrays must be 4-byte aligned");
+  if (batch > 1 && (table_stride < max_pages || dst_stride < dst_pages))
+    return fail(CLOVE_ERR_INVALID_ARG, "a row stride is smaller than the row");
+  const long long capacity = static_cast<long long>(max_pages) * cache->page_size;
+  if (capacity > INT_MAX - 16384) return fail(CLOVE_ERR_UNSUPPORTED, "page table rows name over 2^31 tokens");
+  DeviceInfo dev;
+  rc = current_device(&dev);
+  if (rc) return rc;
+  p.page_table = page_table;
+  p.seq_lens = seq_lens;
+  p.dst_table = dst_table;
+  p.table_stride = table_stride;
+  p.dst_stride = dst_stride;
+  p.capacity = static_cast<int>(capacity);
+  p.batch = batch;
+  p.budget = budget;
+  p.recent = recent;
+  p.key_weights = key_weights;
+  p.kept = kept;
+  p.new_lens = new_lens;
+  p.elem = cache->dtype == CLOVE_DTYPE_E4M3 ? 1 : 2;
+  p.row_bytes = cache->head_dim * p.elem;
+  return launch_evict_cache(p, dev, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

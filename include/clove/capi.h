@@ -17,6 +17,8 @@
  *   clove_gemm_int4        clove::gemm_int4          gemm.cuh:77-87, gemm_int4.cu:195-216
  *   clove_gemm_fp16_batched clove::gemm_fp16_batched gemm.cuh:93-101, gemm_fp16.cu:366-383
  *   clove_flash_attention  clove::flash_attention    attention.cuh:44-56, attention.cu:93-310
+ *   clove_paged_attention  paged_attention (declared only) attention.cuh:85-100
+ *   clove_qk_norm_rope     clove::apply_rope         attention.cu:30-62 (+ norm, cache append)
  *   clove_debug_*          (test hooks: raw int32 accumulators for bit-exact checks)
  *   clove_nsplit_*         (extension: N-split over the GPUs of one node, NCCL all-gather)
  */
@@ -51,7 +53,9 @@ const char* clove_last_error_string(void);
 /* Reads and clears the device-side error word of the current device (a kernel
  * whose bounded wait expired sets it). Synchronises the device. *code = 0 when
  * no kernel reported an error, 1 when a bounded wait expired (mbarrier or
- * cross-rank flag), 2 when a kernel was launched with a shape it rejects. After an
+ * cross-rank flag), 2 when a kernel was launched with a shape it rejects, 3 when a
+ * position, cache slot, page number or sequence length lay outside its range (it was
+ * not followed; the entry point says what was done instead). After an
  * error it also resets the library's kept stream-K state, so call it before
  * further GEMMs once a kernel may have failed. */
 int clove_get_device_error(int* code);
@@ -144,6 +148,97 @@ int clove_quantize_int4(const void* W, int rows, int K, uint8_t* codes, void* sc
 int clove_flash_attention(const void* Q, const void* K, const void* V, void* O, int batch,
                           int num_heads, int num_kv_heads, int seq_len, int head_dim, float scale,
                           int causal, int layout, void* stream);
+
+/* ------------------------------------------------------------------------- */
+/* Paged key-value cache: the decode step's operators.                          */
+/*                                                                             */
+/* K and V live in pages of page_size tokens (a power of two) anywhere in one   */
+/* buffer each; token slot s is row s % page_size of page s / page_size.        */
+/* Strides in elements, the same for K and V: the innermost (head_dim) is 1,    */
+/* the others any multiple of 16 bytes, e.g. [pages, page_size, heads, D] or    */
+/* [pages, heads, page_size, D]. dtype: the operands' 16-bit type, or e4m3 (8   */
+/* bits; a stored value x stands for x * k_scale or x * v_scale; the scales are */
+/* 1 for 16-bit caches). head_dim 64, 128 or 256.                               */
+/* Index arrays are int32 on the device and are read there: sequences may grow  */
+/* between the replays of a captured call. An index outside its range is never  */
+/* followed; the kernel sets device error 3 (clove_get_device_error).           */
+/* ------------------------------------------------------------------------- */
+#define CLOVE_DTYPE_F16 0
+#define CLOVE_DTYPE_BF16 1
+#define CLOVE_DTYPE_E4M3 2
+
+typedef struct {
+  void* K;
+  void* V;
+  int num_pages;
+  int page_size;
+  int num_kv_heads;
+  int head_dim;
+  long long page_stride;
+  long long token_stride;
+  long long head_stride;
+  int dtype;
+  float k_scale;
+  float v_scale;
+} clove_paged_cache;
+
+/* Per-head RMS norm of queries and keys, position rotation, and the append of keys and
+ * values to the cache, in one pass (the reference rotates in place in a kernel of its own,
+ * src/kernels/attention.cu:30-62, and has no query/key norm and no cache append).
+ * Q [num_tokens, num_heads, D], K and V [num_tokens, num_kv_heads, D] of type `dtype`,
+ * token t at t * *_stride elements (multiples of 8: column blocks of a fused projection).
+ * y = x / sqrt(mean(x^2) + eps) * weight per head, weights [D] of the same type (both
+ * NULL: no norm); then pair (i, i + rotary_dim/2), or (2i, 2i + 1) when interleaved, of
+ * the first rotary_dim elements is turned by row positions[t] of rope_table [table_len,
+ * rotary_dim] fp32: rotary_dim/2 cosines, then as many sines. fp32, rounded once.
+ * Q_out (may be Q with the same stride) gets the queries, K_out (may be K, or NULL with a
+ * cache) the keys; with a cache, K and V rows also go to slot slots[t] (a negative slot:
+ * not stored; distinct slots otherwise). A token with a negative position is padding:
+ * nothing of it is written. A position >= table_len is treated the same and reported
+ * (device error 3), a slot outside the cache is not stored and reported. */
+int clove_qk_norm_rope(const void* Q, const void* K, const void* V, long long q_stride,
+                       long long k_stride, long long v_stride, const void* q_weight,
+                       const void* k_weight, float eps, const float* rope_table, int table_len,
+                       int rotary_dim, int interleaved, const int* positions,
+                       const clove_paged_cache* cache, const int* slots, void* Q_out,
+                       long long q_out_stride, void* K_out, long long k_out_stride, int num_tokens,
+                       int num_heads, int num_kv_heads, int head_dim, int dtype, void* stream);
+
+/* Attention of one new token per sequence over its cached keys (the reference declares
+ * paged_attention, include/clove/kernels/attention.cuh:85-100, and never defines it).
+ * Q, O [batch, num_heads, D] with row strides in elements (multiples of 8; head h reads kv
+ * head h / (num_heads / num_kv_heads)); page_table [batch, max_pages], rows table_stride
+ * apart; seq_lens [batch] counts the keys to attend to, the new token's among them. window
+ * > 0: only the last `window` keys (pages before them are not looked up). lse (may be
+ * NULL) [batch, num_heads]: log-sum-exp of the scaled scores. A length of 0 gives zeros
+ * and -inf. A length outside [0, max_pages * page_size] is clamped and reported; a page
+ * outside the cache reads as zeros and is reported (device error 3).
+ * key_weights (may be NULL) [num_pages, num_kv_heads, page_size] fp32: each attended key's
+ * softmax weight, summed over its query heads, is written there, or added when accumulate
+ * != 0; no other entry is touched. No page may then appear in two sequences. It takes
+ * batch * num_heads * max_pages * page_size * 4 bytes of scratch.
+ * Scratch is stream-ordered, from a pool that the library keeps. */
+int clove_paged_attention(const void* Q, long long q_stride, const clove_paged_cache* cache,
+                          const int* page_table, long long table_stride, int max_pages,
+                          const int* seq_lens, void* O, long long o_stride, float* lse,
+                          float* key_weights, int accumulate, int batch, int num_heads, float scale,
+                          int window, int dtype, void* stream);
+
+/* Eviction by key weight (no counterpart in the reference). Per sequence b of n =
+ * seq_lens[b] keys and per kv head: n <= budget keeps all keys; otherwise the last
+ * `recent` (<= budget) keys, and of those before them the budget - recent with the largest
+ * key_weights [num_pages, num_kv_heads, page_size] (ties: the lowest index; NaN counts as
+ * the largest). kept [batch, num_kv_heads, budget] gets their indices in order, -1 behind
+ * them, new_lens [batch] min(n, budget); row j of K, V and key_weights goes to token j of
+ * dst_table [batch, dst_pages]. Every sequence needs fresh pages there for min(n, budget)
+ * tokens: none of them may be a page that a sequence's page_table row still names, or
+ * stand twice. The old pages keep their contents. A length outside the table is clamped,
+ * a bad source page counts as weight 0, a row from or to a bad page is not copied; all are
+ * reported (device error 3). */
+int clove_evict_cache(const clove_paged_cache* cache, float* key_weights, const int* page_table,
+                      long long table_stride, int max_pages, const int* seq_lens, const int* dst_table,
+                      long long dst_stride, int dst_pages, int* kept, int* new_lens, int batch, int budget,
+                      int recent, void* stream);
 
 /* ------------------------------------------------------------------------- */
 /* Test hooks: exact int32 accumulators through the same kernels.              */
