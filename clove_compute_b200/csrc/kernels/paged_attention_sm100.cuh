@@ -22,13 +22,15 @@
 //   (or head elements) as the 16 rows and 8 query heads as the columns: a group of up to 8
 //   heads wastes nothing that costs time. (tcgen05 wants 64 or 128 rows of queries.)
 //   K and V reach the instructions by ldmatrix from XOR-swizzled rows; e4m3 elements are
-//   widened in registers. P is passed as the sum of two 16-bit halves, so that no weight
+//   widened to fp16 in registers. P is passed as the sum of two 16-bit halves, so that no weight
 //   is rounded; scores, maxima, totals and O stay in fp32.
 // * Softmax. Running maximum and total per warp; the maximum is reduced over the warp
 //   only when some lane's score exceeds it.
 #pragma once
 
 #include <cuda_runtime.h>
+
+#include <type_traits>
 
 #include "paged_cache.cuh"
 
@@ -52,6 +54,8 @@ struct PagedShape {
   static constexpr int OPITCH = D + 4;             // floats; conflict-free column writes
   static constexpr int MERGE = kPagedWarps * 8 * OPITCH * 4;
   static constexpr int SMEM = kPagedWarps * RING + MERGE + kPagedWarps * HEADS * 2 * 4;
+  // 8 rows of a chunk read by one ldmatrix phase fall into different banks.
+  __host__ __device__ static constexpr int swizzle(int r) { return CPR >= 8 ? (r & 7) : ((r >> 1) & 3); }
   static constexpr int CTAS_PER_SM = 2 * (SMEM + 1024) <= 228 * 1024 ? 2 : 1;
 };
 
@@ -66,10 +70,6 @@ struct Pair<__half> {
   }
   __device__ static __forceinline__ float2 unpack(uint32_t v) {
     return __half22float2(*reinterpret_cast<const __half2*>(&v));
-  }
-  __device__ static __forceinline__ uint32_t from_e4m3(uint16_t v) {
-    const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2(v, __NV_E4M3);
-    return static_cast<uint32_t>(r.x) | (static_cast<uint32_t>(r.y) << 16);
   }
   __device__ static __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                              uint32_t b1) {
@@ -89,11 +89,6 @@ struct Pair<__nv_bfloat16> {
   __device__ static __forceinline__ float2 unpack(uint32_t v) {
     return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
   }
-  // Exact: every e4m3 value is a bf16 value.
-  __device__ static __forceinline__ uint32_t from_e4m3(uint16_t v) {
-    const float2 f = Pair<__half>::unpack(Pair<__half>::from_e4m3(v));
-    return pack(f.x, f.y);
-  }
   __device__ static __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                              uint32_t b1) {
     asm volatile(
@@ -103,6 +98,12 @@ struct Pair<__nv_bfloat16> {
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
 };
+
+// Two e4m3 values as two fp16 values (exact).
+__device__ __forceinline__ uint32_t e4m3_to_half2(uint16_t v) {
+  const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2(v, __NV_E4M3);
+  return static_cast<uint32_t>(r.x) | (static_cast<uint32_t>(r.y) << 16);
+}
 
 __device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -155,59 +156,55 @@ __device__ __forceinline__ void paged_next_item(const PagedAttnParams& p, PagedC
   } while (c.s.tiles == 0);
 }
 
-// The total number of tiles, and (warp-uniform) the cursor of tile `begin(total)` for this
-// CTA. Lane l sums the sequences [l R, (l+1) R); the lane that holds the tile is found by
-// a scan and its sequences are scanned again in strips of 32.
-__device__ __forceinline__ long long paged_total(const PagedAttnParams& p, int hh_n, int per_lane,
-                                                 long long* lane_sum) {
+// Inclusive sum over the warp's lanes.
+__device__ __forceinline__ int warp_scan(int v) {
   const int lane = static_cast<int>(dev::lane_idx());
-  long long sum = 0;
-  const int b0 = lane * per_lane, b1 = min(p.batch, b0 + per_lane);
-  for (int b = b0; b < b1; ++b) sum += paged_span(p, b).tiles;
-  sum *= hh_n;
-  *lane_sum = sum;
-  long long total = sum;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  return total;
-}
-__device__ __forceinline__ PagedCursor paged_find(const PagedAttnParams& p, int hh_n, int per_lane,
-                                                  long long lane_sum, long long at) {
-  const int lane = static_cast<int>(dev::lane_idx());
-  long long pre = lane_sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, pre, o);
-    if (lane >= o) pre += v;
+    const int x = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += x;
   }
-  // First lane whose inclusive prefix exceeds `at`.
-  const unsigned above = __ballot_sync(0xffffffffu, pre > at);
+  return v;
+}
+
+// Tiles of the sequences [l R, (l+1) R) of lane l, R = per_lane, times items per sequence.
+// (The host has checked that all tiles together stay below 2^31.)
+__device__ __forceinline__ int paged_lane_tiles(const PagedAttnParams& p, int hh_n, int per_lane) {
+  const int b0 = static_cast<int>(dev::lane_idx()) * per_lane, b1 = min(p.batch, b0 + per_lane);
+  int sum = 0;
+  for (int b = b0; b < b1; ++b) sum += paged_span(p, b).tiles;
+  return sum * hh_n;
+}
+
+// The (warp-uniform) cursor of tile `at`; own, upto: this lane's tiles and their inclusive
+// sum. The lane that holds the tile names 32 R sequences, which are scanned in strips.
+__device__ __forceinline__ PagedCursor paged_find(const PagedAttnParams& p, int hh_n, int per_lane,
+                                                  int own, int upto, int at) {
+  const int lane = static_cast<int>(dev::lane_idx());
+  const unsigned above = __ballot_sync(0xffffffffu, upto > at);
   const int owner = above ? __ffs(above) - 1 : 31;
-  long long before = __shfl_sync(0xffffffffu, pre - lane_sum, owner);
-  PagedCursor c{p.batch, 0, 0, {0, 0, 0, 0}};
-  const int b_end = min(p.batch, (owner + 1) * per_lane);
-  for (int b0 = owner * per_lane; b0 < b_end; b0 += 32) {
-    const int b = b0 + lane;
-    const long long t = b < b_end ? static_cast<long long>(paged_span(p, b).tiles) * hh_n : 0;
-    long long inc = t;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += v;
+  int before = __shfl_sync(0xffffffffu, upto - own, owner);
+  int b = owner;
+  if (per_lane > 1) {
+    const int b_end = min(p.batch, (owner + 1) * per_lane);
+    for (int b0 = owner * per_lane; b0 < b_end; b0 += 32) {
+      const int t = b0 + lane < b_end ? paged_span(p, b0 + lane).tiles * hh_n : 0;
+      const int inc = warp_scan(t);
+      const unsigned hit = __ballot_sync(0xffffffffu, before + inc > at);
+      if (hit) {
+        const int l = __ffs(hit) - 1;
+        before += __shfl_sync(0xffffffffu, inc - t, l);
+        b = b0 + l;
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, inc, 31);
     }
-    const unsigned hit = __ballot_sync(0xffffffffu, before + inc > at);
-    if (hit) {
-      const int l = __ffs(hit) - 1;
-      const long long start = before + __shfl_sync(0xffffffffu, inc - t, l);
-      c.b = b0 + l;
-      c.s = paged_span(p, c.b);
-      const long long in = at - start;
-      c.hh = static_cast<int>(in / c.s.tiles);
-      c.tile = static_cast<int>(in - static_cast<long long>(c.hh) * c.s.tiles);
-      return c;
-    }
-    before += __shfl_sync(0xffffffffu, inc, 31);
   }
+  PagedCursor c;
+  c.b = b;
+  c.s = paged_span(p, b);
+  c.hh = (at - before) / c.s.tiles;
+  c.tile = at - before - c.hh * c.s.tiles;
   return c;
 }
 
@@ -216,9 +213,11 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
                                   PagedShape<F8, D, NT>::CTAS_PER_SM)
     paged_attention_kernel(const PagedAttnParams p) {
   using S = PagedShape<F8, D, NT>;
-  using P2 = Pair<T>;
+  // e4m3 elements (and their queries) are multiplied as fp16, whatever the query type.
+  using MT = typename std::conditional<F8, __half, T>::type;
+  using P2 = Pair<MT>;
   constexpr int ROWB = S::ROWB, CPR = S::CPR, KK = D / 16;
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ __align__(1024) uint8_t smem[];
   float* merge = reinterpret_cast<float*>(smem + kPagedWarps * S::RING);
   float* sm_m = merge + S::MERGE / 4;         // [warp][HEADS]
   float* sm_l = sm_m + kPagedWarps * S::HEADS;
@@ -236,7 +235,7 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
   for (int b = cta; b < p.batch; b += static_cast<int>(gridDim.x)) {
     const int n = p.seq_lens[b];
     if ((n < 0 || n > p.capacity) && threadIdx.x == 0) dev::record_error(dev::kDevErrBadIndex);
-    if (n > 0) continue;
+    if (min(n, p.capacity) > 0) continue;
     T* o = static_cast<T*>(p.o) + b * p.o_stride;
     for (int i = static_cast<int>(threadIdx.x) * 8; i < p.heads * D; i += S::THREADS * 8)
       *reinterpret_cast<uint4*>(o + i) = make_uint4(0u, 0u, 0u, 0u);
@@ -246,23 +245,23 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
   }
 
   const int per_lane = (p.batch + 31) / 32;
-  long long lane_sum;
-  const long long total = paged_total(p, hh_n, per_lane, &lane_sum);
-  const long long workers = min(static_cast<long long>(gridDim.x), total);
-  int* meta = p.meta + cta * kPagedMeta;
+  const int own = paged_lane_tiles(p, hh_n, per_lane), upto = warp_scan(own);
+  const int total = __shfl_sync(0xffffffffu, upto, 31);
+  const int workers = min(static_cast<int>(gridDim.x), total);
+  int4* meta = reinterpret_cast<int4*>(p.meta) + cta;
   if (cta >= workers) {
-    if (threadIdx.x == 0) meta[0] = -1, meta[2] = -1;
+    if (threadIdx.x == 0) *meta = make_int4(-1, 0, -1, 0);
     return;
   }
-  const long long t_begin = cta * total / workers, t_end = (cta + 1) * total / workers;
-  const int n_tiles = static_cast<int>(t_end - t_begin);
-  PagedCursor cur = paged_find(p, hh_n, per_lane, lane_sum, t_begin);
+  // Every worker takes total / workers tiles, the first total % workers one more.
+  const int share = total / workers, more = total - share * workers;
+  const int n_tiles = share + (cta < more ? 1 : 0);
+  PagedCursor cur = paged_find(p, hh_n, per_lane, own, upto, cta * share + min(cta, more));
   PagedCursor ld = cur;  // the loads' place
   int ld_left = n_tiles;
   const int page_mask = (1 << p.cache.page_shift) - 1;
   const bool whole_pages = p.cache.page_shift >= 4;  // a 16-key chunk lies in one page
 
-  // Page of the chunk that is loaded next, read one step ahead of its use.
   auto chunk_key = [&](const PagedCursor& c) { return c.s.base + c.tile * kPagedTile + warp * 16; };
   auto page_of = [&](int b, int key) {
     const int pg = p.page_table[b * p.table_stride + (key >> p.cache.page_shift)];
@@ -270,38 +269,47 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
     dev::record_error(dev::kDevErrBadIndex);
     return -1;
   };
-  int ld_page = 0;
+  // Page of the chunk that is loaded next, read one step ahead of its use.
+  int ld_page = -1;
   auto fetch_page = [&]() {
     const int key = chunk_key(ld);
     if (whole_pages && ld_left > 0 && key < ld.s.len) ld_page = page_of(ld.b, key);
   };
+  // Byte strides, and this lane's part of the addresses: a chunk is loaded RPI rows at a
+  // time, CPR lanes per row; 16-byte piece c of row r lies at piece c ^ swizzle(r).
+  constexpr int EB = F8 ? 1 : 2, RPI = 32 / CPR;
+  const long long tok_b = p.cache.token_stride * EB;
+  const long long v_minus_k = static_cast<const uint8_t*>(p.cache.V) - static_cast<const uint8_t*>(p.cache.K);
+  const int ld_row = lane / CPR, piece = lane % CPR;
+  const uint8_t* ld_base = static_cast<const uint8_t*>(p.cache.K) + ld_row * tok_b + piece * 16;
+  const uint32_t ld_dst = ring + ld_row * ROWB + ((piece ^ S::swizzle(ld_row)) << 4);
   auto issue = [&](int stage) {
     if (ld_left > 0) {
       const int key = chunk_key(ld);
       if (key < ld.s.len) {
-        const uint32_t kdst = ring + stage * 2 * S::CHUNK, vdst = kdst + S::CHUNK;
-        const int piece = lane % CPR;
-        const long long head_off = (ld.hh / p.blocks) * p.cache.head_stride;
-        const uint8_t* kb = static_cast<const uint8_t*>(p.cache.K);
-        const uint8_t* vb = static_cast<const uint8_t*>(p.cache.V);
-        constexpr int EB = F8 ? 1 : 2;
-        const bool full = key >= ld.s.first && key + 16 <= ld.s.len;
+        const uint32_t dst = ld_dst + stage * 2 * S::CHUNK;
+        const uint8_t* src = ld_base + (ld.hh / p.blocks) * p.cache.head_stride * EB;
+        if (whole_pages && ld_page >= 0 && key >= ld.s.first && key + 16 <= ld.s.len) {
+          src += ld_page * p.cache.page_stride * EB + (key & page_mask) * tok_b;
 #pragma unroll
-        for (int r0 = 0; r0 < 16; r0 += 32 / CPR) {
-          const int r = r0 + lane / CPR;
-          const int t = key + r;
-          bool ok = full || (t >= ld.s.first && t < ld.s.len);
-          int pg = ld_page;
-          if (!whole_pages && ok) pg = page_of(ld.b, t);
-          ok = ok && pg >= 0;
-          long long off = 0;
-          if (ok)
-            off = (pg * p.cache.page_stride + (t & page_mask) * p.cache.token_stride + head_off) * EB +
-                  piece * 16;
-          const uint32_t sw = CPR >= 8 ? (piece ^ (r & 7)) : (piece ^ ((r >> 1) & 3));
-          const uint32_t d = r * ROWB + sw * 16;
-          cp_async_16(kdst + d, kb + off, ok ? 16u : 0u);
-          cp_async_16(vdst + d, vb + off, ok ? 16u : 0u);
+          for (int i = 0; i < 16 / RPI; ++i) {
+            // swizzle(ld_row + i RPI) = swizzle(ld_row) ^ swizzle(i RPI): ld_row < RPI.
+            const uint32_t d = (dst ^ (S::swizzle(i * RPI) << 4)) + i * RPI * ROWB;
+            cp_async_16(d, src, 16u);
+            cp_async_16(d + S::CHUNK, src + v_minus_k, 16u);
+            src += RPI * tok_b;
+          }
+        } else {
+          for (int i = 0; i < 16 / RPI; ++i) {
+            const int t = key + ld_row + i * RPI;
+            int pg = -1;
+            if (t >= ld.s.first && t < ld.s.len) pg = whole_pages ? ld_page : page_of(ld.b, t);
+            const uint32_t d = (dst ^ (S::swizzle(i * RPI) << 4)) + i * RPI * ROWB;
+            const uint8_t* from =
+                pg < 0 ? src : src + pg * p.cache.page_stride * EB + ((t & page_mask) - ld_row) * tok_b;
+            cp_async_16(d, from, pg < 0 ? 0u : 16u);
+            cp_async_16(d + S::CHUNK, from + v_minus_k, pg < 0 ? 0u : 16u);
+          }
         }
       }
       --ld_left;
@@ -314,6 +322,20 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
 #pragma unroll
   for (int i = 0; i < S::STAGES - 1; ++i) issue(i);
 
+  // ldmatrix addresses within a chunk; piece c is reached by an exclusive or with c << 4.
+  // K (and e4m3 V): lanes 0-15 name rows 0-15 of an even piece, lanes 16-31 of the odd one
+  // behind it. 16-bit V: lanes 0-7, 8-15 rows 0-7 of the even and odd piece, the others
+  // rows 8-15.
+  const uint32_t k_lane = (lane & 15) * ROWB + (((lane >> 4) ^ S::swizzle(lane & 15)) << 4);
+  const int v_row = F8 ? (lane & 15) : (lane & 7) + ((lane >> 4) << 3);
+  const uint32_t v_lane =
+      v_row * ROWB + (((F8 ? lane >> 4 : (lane >> 3) & 1) ^ S::swizzle(v_row)) << 4);
+
+  constexpr bool SCALED_Q = F8 && !std::is_same<T, MT>::value;
+  float q_scale[NT][2];
+  if (!SCALED_Q)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) q_scale[nt][0] = q_scale[nt][1] = p.scale_log2;
   uint32_t qf[NT][KK][2];
   float o[NT][KK][4], m[NT][2], l[NT][2];
   int stage = 0;
@@ -332,17 +354,43 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const int n = nt * 8 + row4;
+        // The k order within 16 elements follows the K fragments (below).
+        const T* x = q + static_cast<long long>(n) * D + (F8 ? 4 : 2) * col4;
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) {
           qf[nt][kk][0] = qf[nt][kk][1] = 0u;
           if (n < live_heads) {
-            // The k order within 16 elements follows the K fragments: see below.
-            const T* x = q + static_cast<long long>(n) * D + kk * 16 + (F8 ? 4 : 2) * col4;
-            qf[nt][kk][0] = *reinterpret_cast<const uint32_t*>(x);
-            qf[nt][kk][1] = *reinterpret_cast<const uint32_t*>(x + (F8 ? 2 : 8));
+            qf[nt][kk][0] = *reinterpret_cast<const uint32_t*>(x + kk * 16);
+            qf[nt][kk][1] = *reinterpret_cast<const uint32_t*>(x + kk * 16 + (F8 ? 2 : 8));
           }
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[nt][kk][e] = 0.f;
+        }
+        if (SCALED_Q) {
+          // bf16 queries as fp16: each head's row is first multiplied by the power of two
+          // that brings its largest element to [1, 2) (exact; elements below 2^-24 of the
+          // largest vanish, as they would in the fp32 sum), its scores by the inverse.
+          uint32_t big = 0u;
+#pragma unroll
+          for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              big = max(big, max(qf[nt][kk][e] & 0x7fff0000u, (qf[nt][kk][e] << 16) & 0x7fff0000u));
+          big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+          big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+          uint32_t ex = big >> 23;  // biased exponent; zero rows, infinities and NaN unscaled
+          ex = ex == 0u || ex == 255u ? 127u : min(ex, 253u);
+          const float down = __uint_as_float((254u - ex) << 23);
+#pragma unroll
+          for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float2 f = Pair<__nv_bfloat16>::unpack(qf[nt][kk][e]);
+              qf[nt][kk][e] = P2::pack(f.x * down, f.y * down);
+            }
+          const float up = __uint_as_float(ex << 23) * p.scale_log2;
+          q_scale[nt][0] = __shfl_sync(0xffffffffu, up, col4 * 8);
+          q_scale[nt][1] = __shfl_sync(0xffffffffu, up, col4 * 8 + 4);
         }
         m[nt][0] = m[nt][1] = __int_as_float(0xff800000);
         l[nt][0] = l[nt][1] = 0.f;
@@ -360,49 +408,47 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) sc[nt][e] = 0.f;
-      // S^T: rows = keys, columns = heads. ldmatrix lane addresses: lanes 0-15 name rows
-      // 0-15 of the left 16 bytes, lanes 16-31 of the right 16 bytes.
-      {
-        const int r = lane & 15;
-        const uint32_t row = ks + r * ROWB;
-        const int sw = CPR >= 8 ? (r & 7) : ((r >> 1) & 3);
+      // S^T: rows = keys, columns = heads.
 #pragma unroll
-        for (int c = 0; c < CPR; c += 2) {
-          uint32_t a[4];
-          ldsm_x4(a, row + (((c + (lane >> 4)) ^ sw) << 4));
-          if (!F8) {
+      for (int c = 0; c < CPR; c += 2) {
+        uint32_t a[4];
+        ldsm_x4(a, (ks + k_lane) ^ (c << 4));
+        if (!F8) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) P2::mma(sc[nt], a, qf[nt][c / 2][0], qf[nt][c / 2][1]);
-          } else {
-            // A lane holds four consecutive elements of a row: the first two stand in for
-            // k = 2c, 2c+1 and the others for k = 2c+8, 2c+9, in Q's fragments alike.
+          for (int nt = 0; nt < NT; ++nt) P2::mma(sc[nt], a, qf[nt][c / 2][0], qf[nt][c / 2][1]);
+        } else {
+          // A lane holds four consecutive elements of a row: the first two stand in for
+          // k = 2c, 2c+1 and the others for k = 2c+8, 2c+9, in Q's fragments alike.
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
-              uint32_t x[4];
-              x[0] = P2::from_e4m3(static_cast<uint16_t>(a[2 * w]));
-              x[1] = P2::from_e4m3(static_cast<uint16_t>(a[2 * w + 1]));
-              x[2] = P2::from_e4m3(static_cast<uint16_t>(a[2 * w] >> 16));
-              x[3] = P2::from_e4m3(static_cast<uint16_t>(a[2 * w + 1] >> 16));
+          for (int w = 0; w < 2; ++w) {
+            uint32_t x[4];
+            x[0] = e4m3_to_half2(static_cast<uint16_t>(a[2 * w]));
+            x[1] = e4m3_to_half2(static_cast<uint16_t>(a[2 * w + 1]));
+            x[2] = e4m3_to_half2(static_cast<uint16_t>(a[2 * w] >> 16));
+            x[3] = e4m3_to_half2(static_cast<uint16_t>(a[2 * w + 1] >> 16));
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) P2::mma(sc[nt], x, qf[nt][c + w][0], qf[nt][c + w][1]);
-            }
+            for (int nt = 0; nt < NT; ++nt) P2::mma(sc[nt], x, qf[nt][c + w][0], qf[nt][c + w][1]);
           }
         }
       }
       const int t0 = key + row4, t1 = t0 + 8;
       const bool full = key >= cur.s.first && key + 16 <= cur.s.len;
-      const bool ok0 = full || (t0 >= cur.s.first && t0 < cur.s.len);
-      const bool ok1 = full || (t1 >= cur.s.first && t1 < cur.s.len);
       bool up = false;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          sc[nt][e] *= p.scale_log2;
-          if (!(e < 2 ? ok0 : ok1)) sc[nt][e] = __int_as_float(0xff800000);
-        }
-        up = up || fmaxf(sc[nt][0], sc[nt][2]) > m[nt][0] || fmaxf(sc[nt][1], sc[nt][3]) > m[nt][1];
+        for (int e = 0; e < 4; ++e) sc[nt][e] *= q_scale[nt][e & 1];
+      if (!full) {
+        const bool ok0 = t0 >= cur.s.first && t0 < cur.s.len, ok1 = t1 >= cur.s.first && t1 < cur.s.len;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!(e < 2 ? ok0 : ok1)) sc[nt][e] = __int_as_float(0xff800000);
       }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        up = up || fmaxf(sc[nt][0], sc[nt][2]) > m[nt][0] || fmaxf(sc[nt][1], sc[nt][3]) > m[nt][1];
       if (p.scores != nullptr) {
         float* out = p.scores +
                      ((static_cast<long long>(cur.b) * p.cache.kv_heads + h) * p.capacity) * p.group + g0;
@@ -411,8 +457,9 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int n = nt * 8 + col4 * 2 + (e & 1);
-            if (n < live_heads && (e < 2 ? ok0 : ok1))
-              out[static_cast<long long>(e < 2 ? t0 : t1) * p.group + n] = sc[nt][e];
+            const int t = e < 2 ? t0 : t1;
+            if (n < live_heads && t >= cur.s.first && t < cur.s.len)
+              out[static_cast<long long>(t) * p.group + n] = sc[nt][e];
           }
       }
       if (__any_sync(0xffffffffu, up)) {
@@ -457,13 +504,10 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
       // e4m3: ldmatrix moves pairs of elements; tile row j < 8 is element 16 kk + 2 j, row
       // 8 + j element 16 kk + 2 j + 1.
       if (!F8) {
-        const int r = (lane & 7) + ((lane >> 4) << 3);
-        const uint32_t row = vs + r * ROWB;
-        const int sw = r & 7;
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) {
           uint32_t a[4];
-          ldsm_x4_t(a, row + (((2 * kk + ((lane >> 3) & 1)) ^ sw) << 4));
+          ldsm_x4_t(a, (vs + v_lane) ^ (kk << 5));
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             P2::mma(o[nt][kk], a, ph[nt][0], ph[nt][1]);
@@ -471,22 +515,19 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
           }
         }
       } else {
-        const int r = lane & 15;
-        const uint32_t row = vs + r * ROWB;
-        const int sw = CPR >= 8 ? (r & 7) : ((r >> 1) & 3);
 #pragma unroll
         for (int k2 = 0; k2 < KK; k2 += 2) {
           uint32_t a[4];
-          ldsm_x4_t(a, row + (((k2 + (lane >> 4)) ^ sw) << 4));
+          ldsm_x4_t(a, (vs + v_lane) ^ (k2 << 4));
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
             const uint32_t lo = __byte_perm(a[2 * w], 0u, 0x3120);
             const uint32_t hi = __byte_perm(a[2 * w + 1], 0u, 0x3120);
             uint32_t x[4];
-            x[0] = P2::from_e4m3(static_cast<uint16_t>(lo));
-            x[1] = P2::from_e4m3(static_cast<uint16_t>(lo >> 16));
-            x[2] = P2::from_e4m3(static_cast<uint16_t>(hi));
-            x[3] = P2::from_e4m3(static_cast<uint16_t>(hi >> 16));
+            x[0] = e4m3_to_half2(static_cast<uint16_t>(lo));
+            x[1] = e4m3_to_half2(static_cast<uint16_t>(lo >> 16));
+            x[2] = e4m3_to_half2(static_cast<uint16_t>(hi));
+            x[3] = e4m3_to_half2(static_cast<uint16_t>(hi >> 16));
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               P2::mma(o[nt][k2 + w], x, ph[nt][0], ph[nt][1]);
@@ -584,64 +625,68 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
     else ++cur.tile;
   }
   cp_async_wait<0>();
-  if (threadIdx.x == 0) {
-    meta[0] = cont_item;
-    meta[1] = cont_ends;
-    meta[2] = open_item;
-  }
+  if (threadIdx.x == 0) *meta = make_int4(cont_item, cont_ends, open_item, 0);
 }
 
 // Joins the items that more than one CTA worked on: block c takes the item that CTA c
 // opened and did not finish (if any). Its parts are CTA c's second partial and the first
-// partials of the CTAs behind it, up to the one that ends the item. One warp per head, the
-// parts in order: O = sum_k O_k 2^(m_k - M) / sum_k l_k 2^(m_k - M).
+// partials of the CTAs behind it, up to the one that ends the item:
+// O = sum_k O_k 2^(m_k - M) / sum_k l_k 2^(m_k - M). 32 warps: one per head and group of
+// parts (part k in group k mod GROUPS), the groups' sums added up in order.
 template <typename T, int D, int HEADS>
-__global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p) {
+__global__ void __launch_bounds__(1024) paged_join_kernel(const PagedAttnParams p) {
+  constexpr int GROUPS = 32 / HEADS, V = D / 32;  // V consecutive elements per lane
+  __shared__ float sums[GROUPS][HEADS][D];
+  __shared__ float totals[GROUPS][HEADS];
   const int c = static_cast<int>(blockIdx.x);
-  dev::grid_dependency_wait();
-  const int item = p.meta[c * kPagedMeta + 2];
-  if (item < 0) return;
   const int lane = static_cast<int>(dev::lane_idx());
-  // CTA behind the last contributor: the first one whose first item is this one and ends.
+  const int n = static_cast<int>(dev::warp_idx()) % HEADS, group = static_cast<int>(dev::warp_idx()) / HEADS;
+  const int4* meta = reinterpret_cast<const int4*>(p.meta);
+  dev::grid_dependency_wait();
+  const int item = meta[c].z;
+  // The last contributor: the first CTA behind c whose first item ends there.
   int last = c + 1;
-  for (;; last += 32) {
+  for (;;) {
     const int k = last + lane;
-    const bool end = k < static_cast<int>(gridDim.x) && p.meta[k * kPagedMeta + 1] != 0 &&
-                     p.meta[k * kPagedMeta] == item;
-    const unsigned hit = __ballot_sync(0xffffffffu, end);
+    const int4 x = k < static_cast<int>(gridDim.x) ? meta[k] : make_int4(-1, 1, -1, 0);
+    if (item < 0) return;
+    const unsigned hit = __ballot_sync(0xffffffffu, x.y != 0);
     if (hit) {
       last += __ffs(hit) - 1;
       break;
     }
-    if (last + 32 >= static_cast<int>(gridDim.x)) return;  // not reached: every open item ends
+    last += 32;
   }
+  if (last >= static_cast<int>(gridDim.x)) return;  // not reached: every open item ends
   const int hh_n = p.cache.kv_heads * p.blocks;
   const int b = item / hh_n, hh = item - b * hh_n, h = hh / p.blocks;
   const int g0 = (hh - h * p.blocks) * HEADS;
   const int live_heads = min(HEADS, p.group - g0);
   const int parts = last - c + 1;
-  for (int n = static_cast<int>(dev::warp_idx()); n < live_heads; n += 8) {
-    auto at = [&](int k) {
-      return static_cast<long long>(k == 0 ? 2 * c + 1 : 2 * (c + k)) * HEADS + n;
-    };
-    float top = __int_as_float(0xff800000);
-    for (int k = lane; k < parts; k += 32) top = fmaxf(top, p.part_m[at(k)]);
+  auto at = [&](int k) {
+    return static_cast<long long>(k == 0 ? 2 * c + 1 : 2 * (c + k)) * HEADS + n;
+  };
+  float top = __int_as_float(0xff800000);
+  if (n < live_heads) {
+    float m0 = top, l0 = 0.f;  // of the first 32 parts
+    if (lane < parts) m0 = p.part_m[at(lane)], l0 = p.part_l[at(lane)];
+    top = m0;
+    for (int k = lane + 32; k < parts; k += 32) top = fmaxf(top, p.part_m[at(k)]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    constexpr int V = D / 32;  // consecutive elements per lane: 2, 4 or 8
     float acc[V], sum = 0.f;
 #pragma unroll
     for (int e = 0; e < V; ++e) acc[e] = 0.f;
     for (int k0 = 0; k0 < parts; k0 += 32) {
-      float f = 0.f, fl = 0.f;
-      if (k0 + lane < parts) {
-        const float mk = p.part_m[at(k0 + lane)];
-        f = mk == top ? 1.f : dev::ex2_approx(mk - top);
-        fl = f * p.part_l[at(k0 + lane)];
+      if (k0 > 0) {
+        m0 = __int_as_float(0xff800000), l0 = 0.f;
+        if (k0 + lane < parts) m0 = p.part_m[at(k0 + lane)], l0 = p.part_l[at(k0 + lane)];
       }
+      const float f = k0 + lane < parts ? (m0 == top ? 1.f : dev::ex2_approx(m0 - top)) : 0.f;
+      const float fl = f * l0;
       const int kn = min(32, parts - k0);
-#pragma unroll 4
-      for (int k = 0; k < kn; ++k) {
+#pragma unroll 8
+      for (int k = group; k < kn; k += GROUPS) {
         const float fk = __shfl_sync(0xffffffffu, f, k);
         sum += __shfl_sync(0xffffffffu, fl, k);
         const float* src = p.part_o + at(k0 + k) * D + lane * V;
@@ -653,18 +698,31 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p
         }
       }
     }
-    const float inv = p.v_scale / sum;
-    T* out = static_cast<T*>(p.o) + b * p.o_stride + static_cast<long long>(h * p.group + g0 + n) * D +
-             lane * V;
 #pragma unroll
-    for (int e = 0; e < V; e += 2)
-      *reinterpret_cast<uint32_t*>(out + e) = Pair<T>::pack(acc[e] * inv, acc[e + 1] * inv);
-    if (lane == 0) {
-      const float l2 = top + log2f(sum);
-      const long long i = static_cast<long long>(b) * p.heads + h * p.group + g0 + n;
-      if (p.lse != nullptr) p.lse[i] = l2 * 0.6931471805599453f;
-      if (p.lse2 != nullptr) p.lse2[i] = l2;
-    }
+    for (int e = 0; e < V; ++e) sums[group][n][lane * V + e] = acc[e];
+    if (lane == 0) totals[group][n] = sum;
+  }
+  __syncthreads();
+  if (group > 0 || n >= live_heads) return;
+  float sum = 0.f, acc[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) acc[e] = 0.f;
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g) {
+    sum += totals[g][n];
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] += sums[g][n][lane * V + e];
+  }
+  const float inv = p.v_scale / sum;
+  T* out = static_cast<T*>(p.o) + b * p.o_stride + static_cast<long long>(h * p.group + g0 + n) * D + lane * V;
+#pragma unroll
+  for (int e = 0; e < V; e += 2)
+    *reinterpret_cast<uint32_t*>(out + e) = Pair<T>::pack(acc[e] * inv, acc[e + 1] * inv);
+  if (lane == 0) {
+    const float l2 = top + log2f(sum);
+    const long long i = static_cast<long long>(b) * p.heads + h * p.group + g0 + n;
+    if (p.lse != nullptr) p.lse[i] = l2 * 0.6931471805599453f;
+    if (p.lse2 != nullptr) p.lse2[i] = l2;
   }
 }
 

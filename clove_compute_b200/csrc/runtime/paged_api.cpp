@@ -239,10 +239,11 @@ int clove_paged_attention(const void* Q, long long q_stride, const clove_paged_c
   p.v_scale = p.cache.v_scale;
   p.key_weights = key_weights;
   p.accumulate = accumulate != 0;
-  const long long items = static_cast<long long>(batch) * p.cache.kv_heads * p.blocks;
-  if (items > INT_MAX) return fail(CLOVE_ERR_UNSUPPORTED, "paged_attention: batch x heads exceeds 2^31");
   // As many CTAs as fit at once, or as there can be tiles. The batch's empty rows need one.
-  const long long tiles = items * ((capacity + kern::kPagedTile - 1) / kern::kPagedTile + 1);
+  const double most = static_cast<double>(batch) * p.cache.kv_heads * p.blocks *
+                      static_cast<double>(capacity / kern::kPagedTile + 2);
+  if (most > INT_MAX) return fail(CLOVE_ERR_UNSUPPORTED, "paged_attention: batch x heads x table exceeds 2^31 tiles");
+  const long long tiles = static_cast<long long>(most);
   const int ctas = static_cast<int>(std::min<long long>(paged_attention_max_ctas(D, hb, e4m3, dev), tiles));
   const size_t slots = static_cast<size_t>(ctas) * 2 * hb;
   const size_t part = slots * D * 4, stat = slots * 4, meta = static_cast<size_t>(ctas) * kern::kPagedMeta * 4;
