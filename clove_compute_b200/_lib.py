@@ -110,3 +110,21 @@ def check(rc: int) -> None:
     if rc != CLOVE_OK:
         msg = lib().clove_last_error_string().decode(errors="replace")
         raise CloveError(rc, msg)
+
+
+_fast = None
+
+
+def fastcall():
+    """The CPython entry points of the paged-cache operators (``csrc/binding/fastcall.c``),
+    bound to the loaded library. Raises if they were not built."""
+    global _fast
+    if _fast is None:
+        lib()
+        try:
+            from . import _fastcall
+        except ImportError as e:
+            raise ImportError("_fastcall.so is missing: build it with `python -m clove_compute_b200.build`") from e
+        _fastcall.init(_LIB_PATH)
+        _fast = _fastcall
+    return _fast

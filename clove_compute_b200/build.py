@@ -4,7 +4,8 @@ Every CUDA source is compiled for sm_100a only (``-gencode
 arch=compute_100a,code=sm_100a``); nvcc cross-compiles without a GPU. Objects
 go to ``clove_compute_b200/_build/`` and are rebuilt when a source or any
 header under ``csrc/`` or ``include/`` is newer. Run ``python -m
-clove_compute_b200.build`` (``-v`` prints ptxas register / spill reports).
+clove_compute_b200.build`` (``-v`` prints ptxas register / spill reports). The CPython
+entry points (``csrc/binding/fastcall.c``) become ``_fastcall.so`` beside it.
 """
 from __future__ import annotations
 
@@ -14,12 +15,14 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libclove_b200.so")
+FASTCALL = os.path.join(PKG, "_fastcall.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = [
@@ -61,6 +64,22 @@ def _compile(src: str, verbose: bool) -> str:
     return r.stderr if verbose else ""
 
 
+def _build_fastcall(force: bool) -> None:
+    src = os.path.join(CSRC, "binding", "fastcall.c")
+    newest = max(os.path.getmtime(src), os.path.getmtime(os.path.join(ROOT, "include", "clove", "capi.h")))
+    if not force and os.path.exists(FASTCALL) and os.path.getmtime(FASTCALL) >= newest:
+        return
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if cc is None:
+        raise RuntimeError("no C compiler found")
+    cmd = [cc, "-std=c11", "-O2", "-Wall", "-fPIC", "-shared", "-I" + os.path.join(ROOT, "include"),
+           "-I" + sysconfig.get_path("include"), src, "-o", FASTCALL + ".tmp", "-ldl"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{cc} failed for {src}:\n{r.stdout}\n{r.stderr}")
+    os.replace(FASTCALL + ".tmp", FASTCALL)
+
+
 def build(verbose: bool = False, force: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     srcs = _sources()
@@ -84,6 +103,7 @@ def build(verbose: bool = False, force: bool = False) -> str:
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         os.replace(tmp, LIB)
+    _build_fastcall(force)
     return LIB
 
 

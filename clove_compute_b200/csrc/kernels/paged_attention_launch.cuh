@@ -28,11 +28,7 @@ int launch(kern::PagedAttnParams& p, int ctas, const DeviceInfo& dev, cudaStream
   }
   cudaLaunchAttribute la[1];
   cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(ctas)), S::THREADS, S::SMEM, stream, la);
-  int rc = check_cuda(cudaLaunchKernelEx(&cfg, fn, p), "paged attention launch");
-  if (rc) return rc;
-  cfg = pdl_config(dim3(static_cast<unsigned>(ctas)), 1024, 0, stream, la);
-  rc = check_cuda(cudaLaunchKernelEx(&cfg, &kern::paged_join_kernel<T, D, S::HEADS>, p),
-                  "paged attention join launch");
+  const int rc = check_cuda(cudaLaunchKernelEx(&cfg, fn, p), "paged attention launch");
   if (rc || p.key_weights == nullptr) return rc;
   return launch_paged_key_weights(p, stream);
 }

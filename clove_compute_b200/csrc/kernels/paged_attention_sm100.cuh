@@ -11,10 +11,11 @@
 //   heads); its keys are cut into tiles of 64. All tiles of all items, in order, are dealt
 //   out evenly: CTA c of W takes tiles [c N / W, (c+1) N / W). So ragged batches, a single
 //   long sequence and many short ones all load every SM alike, with at most two unfinished
-//   items per CTA. Those are left as partial sums in a workspace and joined by a second,
-//   programmatically overlapped kernel in a fixed order (results do not depend on timing;
-//   no counters to keep zeroed between calls, nothing that two captured graphs could
-//   share). Lengths are read on the device: one captured launch serves every step.
+//   items per CTA. Those are left as partial sums in a workspace; the CTA that finishes an
+//   item's last part adds the parts up in their order (results do not depend on timing).
+//   Which CTA that is, a wrapping counter says, which is zero again when the item is done.
+//   (A second kernel for the join cost 3 us more per call.) Lengths are read on the device:
+//   one captured launch serves every step.
 // * Loads. Four warps per CTA, each with its own ring of 16-key K and V chunks filled by
 //   16-byte cp.async (any page size, order and strides), no CTA barrier until an item
 //   ends. Two CTAs per SM keep about 128 KB in flight per SM. The ring runs across items.
@@ -135,17 +136,17 @@ __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Place of a CTA in the tile order: item, its sequence and the tile within it.
+// Place in the tile order: sequence, key head, head block of the group, tile of the item.
 struct PagedCursor {
-  int b;     // sequence
-  int hh;    // (key head, head block) within the sequence
-  int tile;  // tile within the item
+  int b, h, block, tile;
   PagedSpan s;
 };
-__device__ __forceinline__ void paged_next_item(const PagedAttnParams& p, PagedCursor& c, int hh_n) {
+__device__ __forceinline__ void paged_next_item(const PagedAttnParams& p, PagedCursor& c) {
   c.tile = 0;
-  if (++c.hh < hh_n) return;
-  c.hh = 0;
+  if (++c.block < p.blocks) return;
+  c.block = 0;
+  if (++c.h < p.cache.kv_heads) return;
+  c.h = 0;
   do {
     ++c.b;
     if (c.b >= p.batch) {
@@ -203,9 +204,82 @@ __device__ __forceinline__ PagedCursor paged_find(const PagedAttnParams& p, int 
   PagedCursor c;
   c.b = b;
   c.s = paged_span(p, b);
-  c.hh = (at - before) / c.s.tiles;
-  c.tile = at - before - c.hh * c.s.tiles;
+  const int hh = (at - before) / c.s.tiles;
+  c.tile = at - before - hh * c.s.tiles;
+  c.h = hh / p.blocks;
+  c.block = hh - c.h * p.blocks;
   return c;
+}
+
+// Four elements of a head's result from their sums v, the maximum and the total.
+template <typename T, int D>
+__device__ __forceinline__ void paged_store(const PagedAttnParams& p, int b, int head, int d, float (&v)[4],
+                                            float top, float sum) {
+  const float inv = p.v_scale / sum;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] *= inv;
+  T* out = static_cast<T*>(p.o) + b * p.o_stride + static_cast<long long>(head) * D + d;
+  *reinterpret_cast<uint2*>(out) = Quad<T>::pack(v);
+  if (d != 0) return;
+  const float l2 = top + log2f(sum);
+  const long long at = static_cast<long long>(b) * p.heads + head;
+  if (p.lse != nullptr) p.lse[at] = l2 * 0.6931471805599453f;
+  if (p.lse2 != nullptr) p.lse2[at] = l2;
+}
+
+// Adds up the partial results of CTAs c0 .. c1 (c0's second, the others' first) with a
+// running maximum, eight parts of two results at a time in flight, and stores the item.
+template <typename T, int D, int HEADS>
+__device__ __forceinline__ void paged_join(const PagedAttnParams& p, int c0, int c1, int live_heads, int b,
+                                           int head0) {
+  constexpr int THREADS = kPagedWarps * 32, BATCH = 8;
+  const int work = live_heads * (D / 4);  // four elements of a head each
+  for (int i0 = static_cast<int>(threadIdx.x); i0 < work; i0 += 2 * THREADS) {
+    float top[2], sum[2] = {0.f, 0.f}, v[2][4] = {};
+    top[0] = top[1] = __int_as_float(0xff800000);
+    for (int c = c0; c <= c1; c += BATCH) {
+      float m[2][BATCH], l[2][BATCH];
+      float4 x[2][BATCH];
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+          const int idx = i0 + w * THREADS, n = idx / (D / 4), d = (idx - n * (D / 4)) * 4;
+          m[w][k] = __int_as_float(0xff800000);
+          l[w][k] = 0.f;
+          x[w][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (idx < work && c + k <= c1) {
+            const int at = (2 * (c + k) + (c + k == c0 ? 1 : 0)) * HEADS + n;
+            m[w][k] = __ldcg(p.part_m + at);
+            l[w][k] = __ldcg(p.part_l + at);
+            x[w][k] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * D + d));
+          }
+        }
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        float t = top[w];
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) t = fmaxf(t, m[w][k]);
+        const float f0 = top[w] == t ? 1.f : dev::ex2_approx(top[w] - t);
+        top[w] = t;
+        sum[w] *= f0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[w][e] *= f0;
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+          const float f = m[w][k] == t ? 1.f : dev::ex2_approx(m[w][k] - t);
+          sum[w] += f * l[w][k];
+          v[w][0] += f * x[w][k].x, v[w][1] += f * x[w][k].y;
+          v[w][2] += f * x[w][k].z, v[w][3] += f * x[w][k].w;
+        }
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const int idx = i0 + w * THREADS, n = idx / (D / 4), d = (idx - n * (D / 4)) * 4;
+      if (idx < work) paged_store<T, D>(p, b, head0 + n, d, v[w], top[w], sum[w]);
+    }
+  }
 }
 
 template <typename T, bool F8, int D, int NT>
@@ -248,15 +322,12 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
   const int own = paged_lane_tiles(p, hh_n, per_lane), upto = warp_scan(own);
   const int total = __shfl_sync(0xffffffffu, upto, 31);
   const int workers = min(static_cast<int>(gridDim.x), total);
-  int4* meta = reinterpret_cast<int4*>(p.meta) + cta;
-  if (cta >= workers) {
-    if (threadIdx.x == 0) *meta = make_int4(-1, 0, -1, 0);
-    return;
-  }
+  if (cta >= workers) return;
   // Every worker takes total / workers tiles, the first total % workers one more.
   const int share = total / workers, more = total - share * workers;
   const int n_tiles = share + (cta < more ? 1 : 0);
-  PagedCursor cur = paged_find(p, hh_n, per_lane, own, upto, cta * share + min(cta, more));
+  const int t_begin = cta * share + min(cta, more);
+  PagedCursor cur = paged_find(p, hh_n, per_lane, own, upto, t_begin);
   PagedCursor ld = cur;  // the loads' place
   int ld_left = n_tiles;
   const int page_mask = (1 << p.cache.page_shift) - 1;
@@ -269,12 +340,6 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
     dev::record_error(dev::kDevErrBadIndex);
     return -1;
   };
-  // Page of the chunk that is loaded next, read one step ahead of its use.
-  int ld_page = -1;
-  auto fetch_page = [&]() {
-    const int key = chunk_key(ld);
-    if (whole_pages && ld_left > 0 && key < ld.s.len) ld_page = page_of(ld.b, key);
-  };
   // Byte strides, and this lane's part of the addresses: a chunk is loaded RPI rows at a
   // time, CPR lanes per row; 16-byte piece c of row r lies at piece c ^ swizzle(r).
   constexpr int EB = F8 ? 1 : 2, RPI = 32 / CPR;
@@ -283,14 +348,35 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
   const int ld_row = lane / CPR, piece = lane % CPR;
   const uint8_t* ld_base = static_cast<const uint8_t*>(p.cache.K) + ld_row * tok_b + piece * 16;
   const uint32_t ld_dst = ring + ld_row * ROWB + ((piece ^ S::swizzle(ld_row)) << 4);
+  // Pages of this warp's chunks, where a chunk lies in one page: lane i holds that of tile
+  // win_tile + i of the item that is being loaded; the next 32, and those of the next item,
+  // are read well before they are needed.
+  PagedCursor nx;
+  int win = -1, win_tile = 0, win_more = -1, win_next = -1;
+  auto window = [&](const PagedCursor& c, int tile) {
+    const int key = c.s.base + (tile + lane) * kPagedTile + warp * 16;
+    return tile + lane < c.s.tiles && key < c.s.len ? page_of(c.b, key) : -1;
+  };
+  const uint8_t* ld_src = nullptr;  // this lane's address in row 0 of page 0 for the item's head
+  auto enter = [&]() {  // `ld` has come to an item; its window is in win
+    win_tile = ld.tile;
+    ld_src = ld_base + ld.h * p.cache.head_stride * EB;
+    if (ld_left > ld.s.tiles - ld.tile) {
+      nx = ld;
+      paged_next_item(p, nx);
+      if (whole_pages) win_next = window(nx, 0);
+    }
+  };
   auto issue = [&](int stage) {
     if (ld_left > 0) {
       const int key = chunk_key(ld);
+      const int at = ld.tile - win_tile;
+      const int page = __shfl_sync(0xffffffffu, win, at & 31);
       if (key < ld.s.len) {
         const uint32_t dst = ld_dst + stage * 2 * S::CHUNK;
-        const uint8_t* src = ld_base + (ld.hh / p.blocks) * p.cache.head_stride * EB;
-        if (whole_pages && ld_page >= 0 && key >= ld.s.first && key + 16 <= ld.s.len) {
-          src += ld_page * p.cache.page_stride * EB + (key & page_mask) * tok_b;
+        const uint8_t* src = ld_src;
+        if (whole_pages && page >= 0 && key >= ld.s.first && key + 16 <= ld.s.len) {
+          src += page * p.cache.page_stride * EB + (key & page_mask) * tok_b;
 #pragma unroll
           for (int i = 0; i < 16 / RPI; ++i) {
             // swizzle(ld_row + i RPI) = swizzle(ld_row) ^ swizzle(i RPI): ld_row < RPI.
@@ -303,7 +389,7 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
           for (int i = 0; i < 16 / RPI; ++i) {
             const int t = key + ld_row + i * RPI;
             int pg = -1;
-            if (t >= ld.s.first && t < ld.s.len) pg = whole_pages ? ld_page : page_of(ld.b, t);
+            if (t >= ld.s.first && t < ld.s.len) pg = whole_pages ? page : page_of(ld.b, t);
             const uint32_t d = (dst ^ (S::swizzle(i * RPI) << 4)) + i * RPI * ROWB;
             const uint8_t* from =
                 pg < 0 ? src : src + pg * p.cache.page_stride * EB + ((t & page_mask) - ld_row) * tok_b;
@@ -313,12 +399,21 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
         }
       }
       --ld_left;
-      if (++ld.tile >= ld.s.tiles) paged_next_item(p, ld, hh_n);
-      fetch_page();
+      if (++ld.tile >= ld.s.tiles) {
+        if (ld_left > 0) {
+          ld = nx;
+          win = win_next;
+          enter();
+        }
+      } else if (whole_pages) {
+        if (at == 15) win_more = window(ld, win_tile + 32);
+        if (at == 31) win = win_more, win_tile += 32;
+      }
     }
     cp_async_commit();
   };
-  fetch_page();
+  if (whole_pages) win = window(ld, ld.tile);
+  enter();
 #pragma unroll
   for (int i = 0; i < S::STAGES - 1; ++i) issue(i);
 
@@ -338,64 +433,72 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
     for (int nt = 0; nt < NT; ++nt) q_scale[nt][0] = q_scale[nt][1] = p.scale_log2;
   uint32_t qf[NT][KK][2];
   float o[NT][KK][4], m[NT][2], l[NT][2];
-  int stage = 0;
-  bool fresh = true;
-  int seg_begin = cur.tile;  // first tile of the current item in this CTA
-  int cont_item = -1, cont_ends = 0, open_item = -1;
-  for (int i = 0; i < n_tiles; ++i) {
-    const int h = cur.hh / p.blocks;
-    const int g0 = (cur.hh - h * p.blocks) * S::HEADS;  // first head of the block in its group
-    const int live_heads = min(S::HEADS, p.group - g0);
-    const int head0 = h * p.group + g0;
-    if (fresh) {
-      fresh = false;
-      seg_begin = cur.tile;
-      const T* q = static_cast<const T*>(p.q) + cur.b * p.q_stride + static_cast<long long>(head0) * D;
+  // The item's queries, as B fragments. The k order within 16 elements follows the K
+  // fragments (below).
+  auto load_q = [&](const PagedCursor& c) {
+    const int live = min(S::HEADS, p.group - c.block * S::HEADS);
+    const T* q = static_cast<const T*>(p.q) + c.b * p.q_stride +
+                 static_cast<long long>(c.h * p.group + c.block * S::HEADS) * D + (F8 ? 4 : 2) * col4;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const int n = nt * 8 + row4;
-        // The k order within 16 elements follows the K fragments (below).
-        const T* x = q + static_cast<long long>(n) * D + (F8 ? 4 : 2) * col4;
+    for (int nt = 0; nt < NT; ++nt) {
+      const int n = nt * 8 + row4;
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-          qf[nt][kk][0] = qf[nt][kk][1] = 0u;
-          if (n < live_heads) {
-            qf[nt][kk][0] = *reinterpret_cast<const uint32_t*>(x + kk * 16);
-            qf[nt][kk][1] = *reinterpret_cast<const uint32_t*>(x + kk * 16 + (F8 ? 2 : 8));
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[nt][kk][e] = 0.f;
+      for (int kk = 0; kk < KK; ++kk) {
+        qf[nt][kk][0] = qf[nt][kk][1] = 0u;
+        if (n < live) {
+          const T* x = q + n * D + kk * 16;
+          qf[nt][kk][0] = *reinterpret_cast<const uint32_t*>(x);
+          qf[nt][kk][1] = *reinterpret_cast<const uint32_t*>(x + (F8 ? 2 : 8));
         }
-        if (SCALED_Q) {
-          // bf16 queries as fp16: each head's row is first multiplied by the power of two
-          // that brings its largest element to [1, 2) (exact; elements below 2^-24 of the
-          // largest vanish, as they would in the fp32 sum), its scores by the inverse.
-          uint32_t big = 0u;
-#pragma unroll
-          for (int kk = 0; kk < KK; ++kk)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-              big = max(big, max(qf[nt][kk][e] & 0x7fff0000u, (qf[nt][kk][e] << 16) & 0x7fff0000u));
-          big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
-          big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
-          uint32_t ex = big >> 23;  // biased exponent; zero rows, infinities and NaN unscaled
-          ex = ex == 0u || ex == 255u ? 127u : min(ex, 253u);
-          const float down = __uint_as_float((254u - ex) << 23);
-#pragma unroll
-          for (int kk = 0; kk < KK; ++kk)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float2 f = Pair<__nv_bfloat16>::unpack(qf[nt][kk][e]);
-              qf[nt][kk][e] = P2::pack(f.x * down, f.y * down);
-            }
-          const float up = __uint_as_float(ex << 23) * p.scale_log2;
-          q_scale[nt][0] = __shfl_sync(0xffffffffu, up, col4 * 8);
-          q_scale[nt][1] = __shfl_sync(0xffffffffu, up, col4 * 8 + 4);
-        }
-        m[nt][0] = m[nt][1] = __int_as_float(0xff800000);
-        l[nt][0] = l[nt][1] = 0.f;
       }
     }
+  };
+  auto scale_q = [&]() {
+    // bf16 queries as fp16: each head's row is first multiplied by the power of two that
+    // brings its largest element to [1, 2) (exact; elements below 2^-24 of the largest
+    // vanish, as they would in the fp32 sum), its scores by the inverse.
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      uint32_t big = 0u;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          big = max(big, max(qf[nt][kk][e] & 0x7fff0000u, (qf[nt][kk][e] << 16) & 0x7fff0000u));
+      big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+      big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+      uint32_t ex = big >> 23;  // biased exponent; zero rows, infinities and NaN unscaled
+      ex = ex == 0u || ex == 255u ? 127u : min(ex, 253u);
+      const float down = __uint_as_float((254u - ex) << 23);
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float2 f = Pair<__nv_bfloat16>::unpack(qf[nt][kk][e]);
+          qf[nt][kk][e] = P2::pack(f.x * down, f.y * down);
+        }
+      const float up = __uint_as_float(ex << 23) * p.scale_log2;
+      q_scale[nt][0] = __shfl_sync(0xffffffffu, up, col4 * 8);
+      q_scale[nt][1] = __shfl_sync(0xffffffffu, up, col4 * 8 + 4);
+    }
+  };
+  auto reset = [&]() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[nt][kk][e] = 0.f;
+      m[nt][0] = m[nt][1] = __int_as_float(0xff800000);
+      l[nt][0] = l[nt][1] = 0.f;
+    }
+  };
+  int stage = 0;
+  int seg_begin = cur.tile;  // first tile of the current item in this CTA
+  load_q(cur);
+  if (SCALED_Q) scale_q();
+  reset();
+  for (int i = 0; i < n_tiles; ++i) {
     cp_async_wait<S::STAGES - 2>();
     __syncwarp();
     issue(stage == 0 ? S::STAGES - 1 : stage - 1);
@@ -450,8 +553,9 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
       for (int nt = 0; nt < NT; ++nt)
         up = up || fmaxf(sc[nt][0], sc[nt][2]) > m[nt][0] || fmaxf(sc[nt][1], sc[nt][3]) > m[nt][1];
       if (p.scores != nullptr) {
+        const int g0 = cur.block * S::HEADS, live_heads = min(S::HEADS, p.group - g0);
         float* out = p.scores +
-                     ((static_cast<long long>(cur.b) * p.cache.kv_heads + h) * p.capacity) * p.group + g0;
+                     ((static_cast<long long>(cur.b) * p.cache.kv_heads + cur.h) * p.capacity) * p.group + g0;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -540,190 +644,104 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
     stage = stage + 1 == S::STAGES ? 0 : stage + 1;
 
     const bool item_ends = cur.tile + 1 == cur.s.tiles;
-    if (item_ends || i + 1 == n_tiles) {
-      // Join the four warps; write the result, or a partial one where the item goes on in
-      // (or came from) another CTA.
-      const bool begins = seg_begin == 0;
-      const bool whole = begins && item_ends;
-      const int item = cur.b * hh_n + cur.hh;
-      const int slot = 2 * cta + (begins ? 1 : 0);
-      if (!whole) {
-        if (begins) open_item = item;
-        else cont_item = item, cont_ends = item_ends ? 1 : 0;
-      }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float v = l[nt][e];
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) v += __shfl_xor_sync(0xffffffffu, v, x);
-          if (row4 == 0) {
-            sm_m[warp * S::HEADS + nt * 8 + col4 * 2 + e] = m[nt][e];
-            sm_l[warp * S::HEADS + nt * 8 + col4 * 2 + e] = v;
-          }
-        }
-      __syncthreads();
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float* mine = merge + warp * 8 * S::OPITCH;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int n = nt * 8 + col4 * 2 + e;
-          float top = sm_m[n];
-#pragma unroll
-          for (int w = 1; w < kPagedWarps; ++w) top = fmaxf(top, sm_m[w * S::HEADS + n]);
-          const float f = m[nt][e] == top ? 1.f : dev::ex2_approx(m[nt][e] - top);
-#pragma unroll
-          for (int kk = 0; kk < KK; ++kk) {
-            const int d0 = kk * 16 + (F8 ? 2 * row4 : row4), d1 = d0 + (F8 ? 1 : 8);
-            mine[(col4 * 2 + e) * S::OPITCH + d0] = o[nt][kk][e] * f;
-            mine[(col4 * 2 + e) * S::OPITCH + d1] = o[nt][kk][e + 2] * f;
-          }
-        }
-        __syncthreads();
-        for (int idx = static_cast<int>(threadIdx.x); idx < 8 * (D / 4); idx += S::THREADS) {
-          const int j = idx / (D / 4), d = (idx - j * (D / 4)) * 4, n = nt * 8 + j;
-          if (n >= live_heads) continue;
-          float top = sm_m[n];
-#pragma unroll
-          for (int w = 1; w < kPagedWarps; ++w) top = fmaxf(top, sm_m[w * S::HEADS + n]);
-          float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int w = 0; w < kPagedWarps; ++w) {
-            const float mw = sm_m[w * S::HEADS + n];
-            sum += sm_l[w * S::HEADS + n] * (mw == top ? 1.f : dev::ex2_approx(mw - top));
-            const float4 x = *reinterpret_cast<const float4*>(merge + (w * 8 + j) * S::OPITCH + d);
-            v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
-          }
-          if (whole) {
-            const float inv = p.v_scale / sum;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] *= inv;
-            T* out = static_cast<T*>(p.o) + cur.b * p.o_stride + static_cast<long long>(head0 + n) * D + d;
-            *reinterpret_cast<uint2*>(out) = Quad<T>::pack(v);
-            if (d == 0) {
-              const float l2 = top + log2f(sum);
-              const long long at = static_cast<long long>(cur.b) * p.heads + head0 + n;
-              if (p.lse != nullptr) p.lse[at] = l2 * 0.6931471805599453f;
-              if (p.lse2 != nullptr) p.lse2[at] = l2;
-            }
-          } else {
-            const long long at = static_cast<long long>(slot) * S::HEADS + n;
-            *reinterpret_cast<float4*>(p.part_o + at * D + d) = make_float4(v[0], v[1], v[2], v[3]);
-            if (d == 0) {
-              p.part_m[at] = top;
-              p.part_l[at] = sum;
-            }
-          }
-        }
-        __syncthreads();
-      }
-      fresh = true;
+    if (!item_ends && i + 1 < n_tiles) {
+      ++cur.tile;
+      continue;
     }
-    if (item_ends) paged_next_item(p, cur, hh_n);
-    else ++cur.tile;
+    // The item (or this CTA's part of it) is done. The next one's queries are on their way
+    // while the four warps' results are joined.
+    const PagedCursor done = cur;
+    const bool whole = seg_begin == 0 && item_ends;
+    const int item_tile = t_begin + i - done.tile;  // the item's first tile in the tile order
+    const int live_heads = min(S::HEADS, p.group - done.block * S::HEADS);
+    const int head0 = done.h * p.group + done.block * S::HEADS;
+    const int slot = 2 * cta + (seg_begin == 0 ? 1 : 0);
+    if (i + 1 < n_tiles) {
+      paged_next_item(p, cur);
+      load_q(cur);
+      seg_begin = 0;
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float v = l[nt][e];
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) v += __shfl_xor_sync(0xffffffffu, v, x);
+        if (row4 == 0) {
+          sm_m[warp * S::HEADS + nt * 8 + col4 * 2 + e] = m[nt][e];
+          sm_l[warp * S::HEADS + nt * 8 + col4 * 2 + e] = v;
+        }
+      }
+    __syncthreads();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float* mine = merge + warp * 8 * S::OPITCH;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int n = nt * 8 + col4 * 2 + e;
+        float top = sm_m[n];
+#pragma unroll
+        for (int w = 1; w < kPagedWarps; ++w) top = fmaxf(top, sm_m[w * S::HEADS + n]);
+        const float f = m[nt][e] == top ? 1.f : dev::ex2_approx(m[nt][e] - top);
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+          const int d0 = kk * 16 + (F8 ? 2 * row4 : row4), d1 = d0 + (F8 ? 1 : 8);
+          mine[(col4 * 2 + e) * S::OPITCH + d0] = o[nt][kk][e] * f;
+          mine[(col4 * 2 + e) * S::OPITCH + d1] = o[nt][kk][e + 2] * f;
+        }
+      }
+      __syncthreads();
+      const int heads_here = min(8, live_heads - nt * 8);
+      for (int idx = static_cast<int>(threadIdx.x); idx < heads_here * (D / 4); idx += S::THREADS) {
+        const int j = idx / (D / 4), d = (idx - j * (D / 4)) * 4, n = nt * 8 + j;
+        float top = sm_m[n];
+#pragma unroll
+        for (int w = 1; w < kPagedWarps; ++w) top = fmaxf(top, sm_m[w * S::HEADS + n]);
+        float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kPagedWarps; ++w) {
+          const float mw = sm_m[w * S::HEADS + n];
+          sum += sm_l[w * S::HEADS + n] * (mw == top ? 1.f : dev::ex2_approx(mw - top));
+          const float4 x = *reinterpret_cast<const float4*>(merge + (w * 8 + j) * S::OPITCH + d);
+          v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
+        }
+        if (whole) {
+          paged_store<T, D>(p, done.b, head0 + n, d, v, top, sum);
+        } else {
+          const long long at = static_cast<long long>(slot) * S::HEADS + n;
+          *reinterpret_cast<float4*>(p.part_o + at * D + d) = make_float4(v[0], v[1], v[2], v[3]);
+          if (d == 0) {
+            p.part_m[at] = top;
+            p.part_l[at] = sum;
+          }
+        }
+      }
+      __syncthreads();
+    }
+    if (!whole) {
+      // Its parts lie with the CTAs c0 .. c1, in that order; the last one to get here joins
+      // them. Each CTA opens one unfinished item at most: c0's counter is the item's.
+      const int item_end = item_tile + done.s.tiles - 1;
+      const int edge = more * (share + 1);
+      const int c0 = item_tile < edge ? item_tile / (share + 1) : more + (item_tile - edge) / share;
+      const int c1 = item_end < edge ? item_end / (share + 1) : more + (item_end - edge) / share;
+      int* last = reinterpret_cast<int*>(sm_m);
+      __threadfence();  // the partial results, before the count
+      __syncthreads();
+      if (threadIdx.x == 0) *last = atomicInc(p.counters + c0, c1 - c0) == static_cast<unsigned>(c1 - c0);
+      __syncthreads();
+      const bool join = *last != 0;
+      __syncthreads();
+      if (join) {
+        __threadfence();
+        paged_join<T, D, S::HEADS>(p, c0, c1, live_heads, done.b, head0);
+      }
+    }
+    if (SCALED_Q) scale_q();
+    reset();
   }
   cp_async_wait<0>();
-  if (threadIdx.x == 0) *meta = make_int4(cont_item, cont_ends, open_item, 0);
-}
-
-// Joins the items that more than one CTA worked on: block c takes the item that CTA c
-// opened and did not finish (if any). Its parts are CTA c's second partial and the first
-// partials of the CTAs behind it, up to the one that ends the item:
-// O = sum_k O_k 2^(m_k - M) / sum_k l_k 2^(m_k - M). 32 warps: one per head and group of
-// parts (part k in group k mod GROUPS), the groups' sums added up in order.
-template <typename T, int D, int HEADS>
-__global__ void __launch_bounds__(1024) paged_join_kernel(const PagedAttnParams p) {
-  constexpr int GROUPS = 32 / HEADS, V = D / 32;  // V consecutive elements per lane
-  __shared__ float sums[GROUPS][HEADS][D];
-  __shared__ float totals[GROUPS][HEADS];
-  const int c = static_cast<int>(blockIdx.x);
-  const int lane = static_cast<int>(dev::lane_idx());
-  const int n = static_cast<int>(dev::warp_idx()) % HEADS, group = static_cast<int>(dev::warp_idx()) / HEADS;
-  const int4* meta = reinterpret_cast<const int4*>(p.meta);
-  dev::grid_dependency_wait();
-  const int item = meta[c].z;
-  // The last contributor: the first CTA behind c whose first item ends there.
-  int last = c + 1;
-  for (;;) {
-    const int k = last + lane;
-    const int4 x = k < static_cast<int>(gridDim.x) ? meta[k] : make_int4(-1, 1, -1, 0);
-    if (item < 0) return;
-    const unsigned hit = __ballot_sync(0xffffffffu, x.y != 0);
-    if (hit) {
-      last += __ffs(hit) - 1;
-      break;
-    }
-    last += 32;
-  }
-  if (last >= static_cast<int>(gridDim.x)) return;  // not reached: every open item ends
-  const int hh_n = p.cache.kv_heads * p.blocks;
-  const int b = item / hh_n, hh = item - b * hh_n, h = hh / p.blocks;
-  const int g0 = (hh - h * p.blocks) * HEADS;
-  const int live_heads = min(HEADS, p.group - g0);
-  const int parts = last - c + 1;
-  auto at = [&](int k) {
-    return static_cast<long long>(k == 0 ? 2 * c + 1 : 2 * (c + k)) * HEADS + n;
-  };
-  float top = __int_as_float(0xff800000);
-  if (n < live_heads) {
-    float m0 = top, l0 = 0.f;  // of the first 32 parts
-    if (lane < parts) m0 = p.part_m[at(lane)], l0 = p.part_l[at(lane)];
-    top = m0;
-    for (int k = lane + 32; k < parts; k += 32) top = fmaxf(top, p.part_m[at(k)]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float acc[V], sum = 0.f;
-#pragma unroll
-    for (int e = 0; e < V; ++e) acc[e] = 0.f;
-    for (int k0 = 0; k0 < parts; k0 += 32) {
-      if (k0 > 0) {
-        m0 = __int_as_float(0xff800000), l0 = 0.f;
-        if (k0 + lane < parts) m0 = p.part_m[at(k0 + lane)], l0 = p.part_l[at(k0 + lane)];
-      }
-      const float f = k0 + lane < parts ? (m0 == top ? 1.f : dev::ex2_approx(m0 - top)) : 0.f;
-      const float fl = f * l0;
-      const int kn = min(32, parts - k0);
-#pragma unroll 8
-      for (int k = group; k < kn; k += GROUPS) {
-        const float fk = __shfl_sync(0xffffffffu, f, k);
-        sum += __shfl_sync(0xffffffffu, fl, k);
-        const float* src = p.part_o + at(k0 + k) * D + lane * V;
-#pragma unroll
-        for (int e = 0; e < V; e += 2) {
-          const float2 x = *reinterpret_cast<const float2*>(src + e);
-          acc[e] += fk * x.x;
-          acc[e + 1] += fk * x.y;
-        }
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < V; ++e) sums[group][n][lane * V + e] = acc[e];
-    if (lane == 0) totals[group][n] = sum;
-  }
-  __syncthreads();
-  if (group > 0 || n >= live_heads) return;
-  float sum = 0.f, acc[V];
-#pragma unroll
-  for (int e = 0; e < V; ++e) acc[e] = 0.f;
-#pragma unroll
-  for (int g = 0; g < GROUPS; ++g) {
-    sum += totals[g][n];
-#pragma unroll
-    for (int e = 0; e < V; ++e) acc[e] += sums[g][n][lane * V + e];
-  }
-  const float inv = p.v_scale / sum;
-  T* out = static_cast<T*>(p.o) + b * p.o_stride + static_cast<long long>(h * p.group + g0 + n) * D + lane * V;
-#pragma unroll
-  for (int e = 0; e < V; e += 2)
-    *reinterpret_cast<uint32_t*>(out + e) = Pair<T>::pack(acc[e] * inv, acc[e + 1] * inv);
-  if (lane == 0) {
-    const float l2 = top + log2f(sum);
-    const long long i = static_cast<long long>(b) * p.heads + h * p.group + g0 + n;
-    if (p.lse != nullptr) p.lse[i] = l2 * 0.6931471805599453f;
-    if (p.lse2 != nullptr) p.lse2[i] = l2;
-  }
 }
 
 }  // namespace kern

@@ -43,9 +43,18 @@ __global__ void __launch_bounds__(256) paged_key_weights_kernel(const PagedAttnP
   }
 }
 
+// Counters of the attention kernel (PagedAttnParams::counters), zero between calls; handed
+// out by the host.
+__device__ unsigned g_paged_counters[kPagedCounters];
+
 }  // namespace kern
 
 namespace rt {
+
+int paged_counter_base(unsigned** out) {
+  return check_cuda(cudaGetSymbolAddress(reinterpret_cast<void**>(out), kern::g_paged_counters),
+                    "cudaGetSymbolAddress(paged counters)");
+}
 
 int launch_paged_key_weights(const kern::PagedAttnParams& p, cudaStream_t stream) {
   const long long rows = static_cast<long long>(p.batch) * p.cache.kv_heads;

@@ -46,7 +46,7 @@ struct RopeParams {
 
 // paged_attention_sm100.cuh
 constexpr int kPagedTile = 64;  // keys per CTA step
-constexpr int kPagedMeta = 4;   // ints of PagedAttnParams::meta per CTA
+constexpr int kPagedCounters = 1 << 18;
 struct PagedAttnParams {
   const void* q;
   void* o;
@@ -62,13 +62,12 @@ struct PagedAttnParams {
   int window;  // 0: all keys
   float scale_log2;  // scale * k_scale * log2(e)
   float v_scale;
-  // Workspace: per CTA two partial results (heads in a block x D sums, maxima, totals)
-  // and what they belong to: {item that its first partial continues or -1, whether the
-  // item ends there, item that its second partial opens or -1}.
+  // Workspace: per CTA two partial results (heads in a block x D sums, maxima, totals) and
+  // one counter, zero before and after the call.
   float* part_o;
   float* part_m;
   float* part_l;
-  int* meta;
+  unsigned* counters;
   // Key weights (null: not asked for): the scores of every key and head, times log2(e),
   // [batch, kv_heads, capacity, group], and each head's log2-sum-exp2 [batch, heads].
   float* scores;

@@ -160,6 +160,8 @@ int launch_paged_attention_f16(kern::PagedAttnParams& p, int head_dim, int heads
                                const DeviceInfo& dev, cudaStream_t stream);
 int launch_paged_attention_bf16(kern::PagedAttnParams& p, int head_dim, int heads, bool e4m3, int ctas,
                                 const DeviceInfo& dev, cudaStream_t stream);
+// Device address of the library's kern::kPagedCounters counters.
+int paged_counter_base(unsigned** out);
 int launch_paged_key_weights(const kern::PagedAttnParams& p, cudaStream_t stream);
 int launch_evict_cache(const kern::EvictParams& p, const DeviceInfo& dev, cudaStream_t stream);
 int read_clear_error_evict();

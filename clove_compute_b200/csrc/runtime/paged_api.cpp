@@ -22,12 +22,8 @@ inline bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintp
 std::mutex g_pool_mu;
 cudaMemPool_t g_pool[64];
 
-int scratch_alloc(void** out, size_t bytes, int device, cudaStream_t s) {
-  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-  int rc = check_cuda(cudaStreamIsCapturing(s, &cap), "cudaStreamIsCapturing");
-  if (rc) return rc;
-  if (cap != cudaStreamCaptureStatusNone)
-    return check_cuda(cudaMallocAsync(out, bytes, s), "cudaMallocAsync(paged attention)");
+int scratch_alloc(void** out, size_t bytes, int device, bool capturing, cudaStream_t s) {
+  if (capturing) return check_cuda(cudaMallocAsync(out, bytes, s), "cudaMallocAsync(paged attention)");
   cudaMemPool_t pool;
   {
     std::lock_guard<std::mutex> lock(g_pool_mu);
@@ -36,7 +32,7 @@ int scratch_alloc(void** out, size_t bytes, int device, cudaStream_t s) {
       props.allocType = cudaMemAllocationTypePinned;
       props.location.type = cudaMemLocationTypeDevice;
       props.location.id = device;
-      rc = check_cuda(cudaMemPoolCreate(&pool, &props), "cudaMemPoolCreate(paged attention)");
+      int rc = check_cuda(cudaMemPoolCreate(&pool, &props), "cudaMemPoolCreate(paged attention)");
       if (rc) return rc;
       uint64_t keep = UINT64_MAX;
       rc = check_cuda(cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep),
@@ -50,6 +46,107 @@ int scratch_alloc(void** out, size_t bytes, int device, cudaStream_t s) {
     pool = g_pool[device & 63];
   }
   return check_cuda(cudaMallocFromPoolAsync(out, bytes, pool, s), "cudaMallocFromPoolAsync(paged attention)");
+}
+
+// Workspace of the attention kernel: per-CTA counters, zero between calls, and partial
+// results. Calls that can overlap on the GPU must not share one:
+// * each stream keeps its own (by the stream's id: a destroyed stream's handle may return
+//   as another stream's, and every thread's default stream has the same handle);
+// * each captured call gets counters that no other call ever gets, and partial results from
+//   the graph's memory, since its graph may be replayed beside anything.
+// Counters come from an array in the library, 1 MB per device (over 800 calls and streams);
+// when it is used up, or its address is not known yet under capture, a call brings its own
+// and clears them first.
+constexpr int kMaxCtas = 1024;
+constexpr size_t kKeptParts = 8u << 20;
+constexpr int kMaxKept = 64;
+struct KeptWorkspace {
+  unsigned long long stream_id;
+  unsigned* counters;
+  float* parts;
+};
+struct DeviceWorkspaces {
+  unsigned* base = nullptr;  // the device's counters
+  int used = 0;
+  int kept_count = 0;
+  KeptWorkspace kept[kMaxKept];
+};
+std::mutex g_ws_mu;
+DeviceWorkspaces g_ws[64];
+
+struct Workspace {
+  unsigned* counters = nullptr;
+  float* parts = nullptr;
+  void* own = nullptr;  // to be released after the call
+  bool capturing = false;
+};
+
+// `count` counters that nobody else has, or null.
+unsigned* reserve_counters(DeviceWorkspaces& d, int count) {
+  if (d.base == nullptr || d.used + count > kern::kPagedCounters) return nullptr;
+  unsigned* c = d.base + d.used;
+  d.used += count;
+  return c;
+}
+
+int take_workspace(Workspace* w, int ctas, size_t part_bytes, int device, cudaStream_t s) {
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  int rc = check_cuda(cudaStreamIsCapturing(s, &cap), "cudaStreamIsCapturing");
+  if (rc) return rc;
+  w->capturing = cap != cudaStreamCaptureStatusNone;
+  if (ctas > kMaxCtas || part_bytes > kKeptParts)
+    return fail(CLOVE_ERR_UNSUPPORTED, "paged_attention: workspace of %d CTAs", ctas);
+  unsigned long long id = 0;
+  if (!w->capturing) {
+    rc = check_cuda(cudaStreamGetId(s, &id), "cudaStreamGetId");
+    if (rc) return rc;
+  }
+  {
+    std::lock_guard<std::mutex> lock(g_ws_mu);
+    DeviceWorkspaces& d = g_ws[device & 63];
+    if (w->capturing) {
+      w->counters = reserve_counters(d, (ctas + 31) & ~31);
+    } else {
+      for (int i = 0; i < d.kept_count; ++i)
+        if (d.kept[i].stream_id == id) {
+          w->counters = d.kept[i].counters;
+          w->parts = d.kept[i].parts;
+          return CLOVE_OK;
+        }
+      if (d.base == nullptr) {
+        rc = paged_counter_base(&d.base);
+        if (rc) return rc;
+      }
+      if (d.kept_count < kMaxKept) {
+        unsigned* c = reserve_counters(d, kMaxCtas);
+        if (c != nullptr) {
+          void* parts = nullptr;
+          rc = scratch_alloc(&parts, kKeptParts, device, false, s);
+          if (rc) return rc;
+          d.kept[d.kept_count++] = KeptWorkspace{id, c, static_cast<float*>(parts)};
+          w->counters = c;
+          w->parts = static_cast<float*>(parts);
+          return CLOVE_OK;
+        }
+      }
+    }
+  }
+  // Partial results, and counters where none were left, for this call alone.
+  const size_t head = w->counters == nullptr ? kMaxCtas * sizeof(unsigned) : 0;
+  rc = scratch_alloc(&w->own, head + part_bytes, device, w->capturing, s);
+  if (rc) return rc;
+  w->parts = reinterpret_cast<float*>(static_cast<char*>(w->own) + head);
+  if (head != 0) {
+    w->counters = static_cast<unsigned*>(w->own);
+    rc = check_cuda(cudaMemsetAsync(w->own, 0, head, s), "cudaMemsetAsync(paged attention)");
+    if (rc) cudaFreeAsync(w->own, s);
+  }
+  return rc;
+}
+
+int drop_workspace(Workspace* w, cudaStream_t s) {
+  if (w->own == nullptr) return CLOVE_OK;
+  return check_cuda(cudaFreeAsync(w->own, s), "cudaFreeAsync(paged attention)");
 }
 
 // Checks a cache description and converts it; `dtype` is the 16-bit type it is used with.
@@ -245,30 +342,32 @@ int clove_paged_attention(const void* Q, long long q_stride, const clove_paged_c
   if (most > INT_MAX) return fail(CLOVE_ERR_UNSUPPORTED, "paged_attention: batch x heads x table exceeds 2^31 tiles");
   const long long tiles = static_cast<long long>(most);
   const int ctas = static_cast<int>(std::min<long long>(paged_attention_max_ctas(D, hb, e4m3, dev), tiles));
-  const size_t slots = static_cast<size_t>(ctas) * 2 * hb;
-  const size_t part = slots * D * 4, stat = slots * 4, meta = static_cast<size_t>(ctas) * kern::kPagedMeta * 4;
   const size_t heads = (static_cast<size_t>(batch) * num_heads * 4 + 255) & ~size_t(255);
   const size_t scores = static_cast<size_t>(batch) * num_heads * static_cast<size_t>(capacity) * 4;
-  size_t bytes = part + 2 * stat + meta;
-  bytes = (bytes + 255) & ~size_t(255);
-  const size_t at_scores = bytes;
-  if (key_weights != nullptr) bytes += heads + scores;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  void* ws = nullptr;
-  rc = scratch_alloc(&ws, bytes, dev.device, s);
+  Workspace ws;
+  rc = take_workspace(&ws, ctas, static_cast<size_t>(ctas) * 2 * hb * (D + 2) * 4, dev.device, s);
   if (rc) return rc;
-  char* w = static_cast<char*>(ws);
-  p.part_o = reinterpret_cast<float*>(w);
-  p.part_m = reinterpret_cast<float*>(w + part);
-  p.part_l = reinterpret_cast<float*>(w + part + stat);
-  p.meta = reinterpret_cast<int*>(w + part + 2 * stat);
+  p.counters = ws.counters;
+  p.part_o = ws.parts;
+  p.part_m = p.part_o + static_cast<size_t>(ctas) * 2 * hb * D;
+  p.part_l = p.part_m + static_cast<size_t>(ctas) * 2 * hb;
+  char* sc = nullptr;
   if (key_weights != nullptr) {
-    p.lse2 = reinterpret_cast<float*>(w + at_scores);
-    p.scores = reinterpret_cast<float*>(w + at_scores + heads);
+    rc = scratch_alloc(reinterpret_cast<void**>(&sc), heads + scores, dev.device, ws.capturing, s);
+    if (!rc) {
+      p.lse2 = reinterpret_cast<float*>(sc);
+      p.scores = reinterpret_cast<float*>(sc + heads);
+    }
   }
-  rc = dtype == CLOVE_DTYPE_F16 ? launch_paged_attention_f16(p, D, hb, e4m3, ctas, dev, s)
-                                : launch_paged_attention_bf16(p, D, hb, e4m3, ctas, dev, s);
-  const int rc2 = check_cuda(cudaFreeAsync(ws, s), "cudaFreeAsync(paged attention)");
+  if (!rc)
+    rc = dtype == CLOVE_DTYPE_F16 ? launch_paged_attention_f16(p, D, hb, e4m3, ctas, dev, s)
+                                  : launch_paged_attention_bf16(p, D, hb, e4m3, ctas, dev, s);
+  if (sc != nullptr) {
+    const int rc2 = check_cuda(cudaFreeAsync(sc, s), "cudaFreeAsync(paged attention scores)");
+    if (!rc) rc = rc2;
+  }
+  const int rc2 = drop_workspace(&ws, s);
   return rc ? rc : rc2;
 }
 

@@ -15,7 +15,7 @@ import ctypes
 
 import torch
 
-from ._lib import PagedCacheStruct, check, lib
+from ._lib import PagedCacheStruct, check, fastcall
 
 DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float8_e4m3fn: 2}
 _16BIT = (torch.float16, torch.bfloat16)
@@ -56,7 +56,7 @@ class PagedCache:
         self.struct = PagedCacheStruct(K.data_ptr(), V.data_ptr(), self.num_pages, self.page_size,
                                        self.num_kv_heads, self.head_dim, K.stride(0), K.stride(tok),
                                        K.stride(head), DTYPES[K.dtype], self.k_scale, self.v_scale)
-        self._ref = ctypes.byref(self.struct)
+        self._address = ctypes.addressof(self.struct)
 
 
 def _ints(t, name, device, shape):
@@ -118,6 +118,12 @@ def _operand(t, name):
         raise ValueError(f"{name} must be 3-D, got shape {tuple(t.shape)}")
 
 
+# The current stream's handle, without the Stream object that torch.cuda.current_stream()
+# builds (2 us a call).
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _on(fn, device, stream, *args):
     """fn(stream handle, *args) with `device` current; an explicit stream is current while
     outputs are allocated, so that their memory belongs to it."""
@@ -127,8 +133,8 @@ def _on(fn, device, stream, *args):
             return fn(s.cuda_stream, *args)
     if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
-            return fn(torch.cuda.current_stream(device).cuda_stream, *args)
-    return fn(torch.cuda.current_stream(device).cuda_stream, *args)
+            return fn(_current_stream(device.index), *args)
+    return fn(_current_stream(device.index), *args)
 
 
 def rope_table(length: int, rotary_dim: int, theta: float = 10000.0, device="cuda") -> torch.Tensor:
@@ -185,7 +191,7 @@ def _qk_norm_rope(stream, Q, K, table, positions, q_weight, k_weight, eps, inter
         if cache.device != device:
             raise ValueError(f"the cache must be on {device}")
         vs = _heads(V, "V", dtype, device, kv)
-        vp, sp, ref = V.data_ptr(), _ints(slots, "slots", device, (T,)), cache._ref
+        vp, sp, ref = V.data_ptr(), _ints(slots, "slots", device, (T,)), cache._address
     elif V is not None or slots is not None:
         raise ValueError("V and slots need a cache")
     if Q_out is None:
@@ -196,10 +202,12 @@ def _qk_norm_rope(stream, Q, K, table, positions, q_weight, k_weight, eps, inter
     if K_out is None and cache is None:
         K_out = torch.empty(kv, dtype=dtype, device=device)
     kos = _heads(K_out, "K_out", dtype, device, kv) if K_out is not None else 0
-    check(lib().clove_qk_norm_rope(
+    rc = fastcall().qk_norm_rope(
         Q.data_ptr(), K.data_ptr(), vp, qs, ks, vs, wq, wk, eps, tp, table.shape[0], table.shape[1],
         1 if interleaved else 0, pp, ref, sp, Q_out.data_ptr(), qos,
-        K_out.data_ptr() if K_out is not None else None, kos, T, H, Hkv, D, DTYPES[dtype], stream))
+        K_out.data_ptr() if K_out is not None else None, kos, T, H, Hkv, D, DTYPES[dtype], stream)
+    if rc:
+        check(rc)
     return Q_out, K_out
 
 
@@ -241,10 +249,12 @@ def _paged_attention(stream, Q, cache, page_table, seq_lens, scale, window, lse,
                      (cache.num_pages, cache.num_kv_heads, cache.page_size))
     elif accumulate:
         raise ValueError("accumulate needs key_weights")
-    check(lib().clove_paged_attention(
-        Q.data_ptr(), qs, cache._ref, pt, page_table.stride(0), page_table.shape[1], sl, O.data_ptr(), os,
+    rc = fastcall().paged_attention(
+        Q.data_ptr(), qs, cache._address, pt, page_table.stride(0), page_table.shape[1], sl, O.data_ptr(), os,
         lp, kw, 1 if accumulate else 0, B, H, D ** -0.5 if scale is None else scale, window,
-        DTYPES[dtype], stream))
+        DTYPES[dtype], stream)
+    if rc:
+        check(rc)
     return O
 
 
@@ -273,7 +283,9 @@ def _evict_cache(stream, cache, key_weights, page_table, seq_lens, dst_table, bu
         raise ValueError("budget must be positive")
     kept = torch.empty((B, cache.num_kv_heads, budget), dtype=torch.int32, device=device)
     new_lens = torch.empty((B,), dtype=torch.int32, device=device)
-    check(lib().clove_evict_cache(
-        cache._ref, kw, pt, page_table.stride(0), page_table.shape[1], sl, dt, dst_table.stride(0),
-        dst_table.shape[1], kept.data_ptr(), new_lens.data_ptr(), B, budget, recent, stream))
+    rc = fastcall().evict_cache(
+        cache._address, kw, pt, page_table.stride(0), page_table.shape[1], sl, dt, dst_table.stride(0),
+        dst_table.shape[1], kept.data_ptr(), new_lens.data_ptr(), B, budget, recent, stream)
+    if rc:
+        check(rc)
     return kept, new_lens
