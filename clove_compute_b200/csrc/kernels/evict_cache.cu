@@ -7,10 +7,12 @@
 //
 // Two kernels. The selection: one cluster per (sequence, key head), each CTA holding a
 // contiguous slice of the weights in shared memory as order-preserving integers, so that
-// they are read once; a radix select of four 8-bit digits over histograms that the CTAs
-// add up through distributed shared memory (one cluster barrier per digit), then an
-// ordered compaction by ballots. Integer counts only: the result does not depend on
-// timing. The copy: bound by memory, 16 bytes per lane, four rows per lane in flight.
+// they are read once; a radix select of three digits (11, 11 and 10 bits: an octave of
+// weights falls into four first digits) over histograms that the CTAs add up through
+// distributed shared memory (one cluster barrier per digit), then an ordered compaction,
+// every warp over a contiguous part of its own. Integer counts only: the result does not
+// depend on timing. The copy: bound by memory, 16 bytes per lane, four rows of K and V per
+// lane in flight while the next rows' places are looked up.
 #include <algorithm>
 #include <atomic>
 
@@ -21,11 +23,12 @@
 namespace clove {
 namespace kern {
 
-constexpr int kEvictThreads = 1024;
+constexpr int kEvictThreads = 512;
 constexpr int kEvictWarps = kEvictThreads / 32;
 // Keys of a slice held in shared memory (96 KB: two CTAs per SM); a longer slice reads the
 // rest again from memory in every pass.
 constexpr int kEvictCached = 24576;
+constexpr int kEvictBins = 2048;
 
 // Larger weight <=> larger integer; -0 equals 0; every NaN above everything.
 __device__ __forceinline__ uint32_t weight_order(float w) {
@@ -34,6 +37,15 @@ __device__ __forceinline__ uint32_t weight_order(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
+__device__ __forceinline__ uint4 ld_cluster_v4(const uint32_t* p, uint32_t rank) {
+  uint4 v;
+  const uint32_t a = dev::map_shared_to_rank(dev::smem_u32(p), rank);
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(a)
+               : "memory");
+  return v;
+}
 __device__ __forceinline__ uint32_t ld_cluster_u32(const uint32_t* p, uint32_t rank) {
   uint32_t v;
   const uint32_t a = dev::map_shared_to_rank(dev::smem_u32(p), rank);
@@ -41,12 +53,13 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(const uint32_t* p, uint32_t r
   return v;
 }
 
+// LONG: slices may exceed kEvictCached keys.
+template <bool LONG>
 __global__ void __launch_bounds__(kEvictThreads, 2) evict_select_kernel(const EvictParams p, int cs) {
   extern __shared__ uint32_t cached[];
-  __shared__ uint32_t hist[2][256];
-  __shared__ uint32_t sums[256];
+  __shared__ __align__(16) uint32_t hist[2][kEvictBins];
   __shared__ uint32_t counts[2];  // this CTA's keys above the threshold, and equal to it
-  __shared__ uint32_t warp_eq[2][kEvictWarps], warp_take[2][kEvictWarps];
+  __shared__ uint32_t warp_a[kEvictWarps], warp_b[kEvictWarps];
   __shared__ uint32_t pick[2];  // chosen digit, keys of larger digits
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = blockIdx.x % cs;
@@ -68,191 +81,251 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_select_kernel(const Ev
       kept[j] = j < n ? j : -1;
     return;  // the whole cluster
   }
-  // Candidates [0, m), `want` of them to keep; slice [s0, s1) of this CTA.
+  // Candidates [0, m), `want` of them to keep; slice [s0, s0 + sn) of this CTA.
   const int m = n - p.recent, want = p.budget - p.recent;
   const int per = (m + cs - 1) / cs;
-  const int s0 = min(m, static_cast<int>(rank) * per), s1 = min(m, s0 + per), sn = s1 - s0;
-  auto load = [&](int t) {
-    const int pg = p.page_table[b * p.table_stride + (t >> p.cache.page_shift)];
-    if (pg < 0 || pg >= p.cache.num_pages) {
-      dev::record_error(dev::kDevErrBadIndex);
-      return weight_order(0.f);
+  const int s0 = min(m, static_cast<int>(rank) * per), sn = min(m, s0 + per) - s0;
+  // Weights of N keys of the slice, kEvictThreads apart, looked up and then read side by
+  // side (no branch between the loads; a bad page counts as weight 0).
+  bool bad = false;
+  auto load = [&](int i0, auto& u) {
+    constexpr int N = sizeof(u) / 4;
+    int pg[N];
+    float w[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int i = i0 + k * kEvictThreads;
+      pg[k] = i < sn ? p.page_table[b * p.table_stride + ((s0 + i) >> p.cache.page_shift)] : 0;
     }
-    return weight_order(p.key_weights[((static_cast<long long>(pg) * p.cache.kv_heads + h)
-                                       << p.cache.page_shift) +
-                                      (t & page_mask)]);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int i = i0 + k * kEvictThreads;
+      const bool ok = pg[k] >= 0 && pg[k] < p.cache.num_pages;
+      bad = bad || !ok;
+      w[k] = 0.f;
+      if (ok && i < sn)
+        w[k] = p.key_weights[((static_cast<long long>(pg[k]) * p.cache.kv_heads + h) << p.cache.page_shift) +
+                             ((s0 + i) & page_mask)];
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) u[k] = weight_order(w[k]);
   };
-  if (tid < 256) hist[0][tid] = 0;
-  const int in_smem = min(sn, kEvictCached);
-#pragma unroll 4
-  for (int i = tid; i < in_smem; i += kEvictThreads) cached[i] = load(s0 + i);
+  for (int i = tid; i < kEvictBins; i += kEvictThreads) hist[0][i] = 0;
+  const int in_smem = LONG ? min(sn, kEvictCached) : sn;
+  for (int i0 = tid; i0 < in_smem; i0 += 8 * kEvictThreads) {
+    uint32_t u[8];
+    load(i0, u);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (i0 + k * kEvictThreads < in_smem) cached[i0 + k * kEvictThreads] = u[k];
+  }
+  if (bad) dev::record_error(dev::kDevErrBadIndex);
   __syncthreads();
-  auto key = [&](int i) { return i < in_smem ? cached[i] : load(s0 + i); };
+  auto key = [&](int i) {
+    if (!LONG || i < in_smem) return cached[i];
+    uint32_t u[1];
+    load(i, u);
+    return u[0];
+  };
 
   uint32_t prefix = 0;  // digits chosen so far
-  uint32_t left = static_cast<uint32_t>(want), above = 0;
-  for (int d = 0; d < 4; ++d) {
-    const int shift = 24 - 8 * d;
+  uint32_t left = static_cast<uint32_t>(want);
+  for (int d = 0; d < 3; ++d) {
+    const int shift = d == 0 ? 21 : d == 1 ? 10 : 0, bits = d == 2 ? 10 : 11;
+    const uint32_t mask = (1u << bits) - 1u;
     uint32_t* mine = hist[d & 1];
-    for (int i = tid; i < sn; i += kEvictThreads) {
-      const uint32_t u = key(i);
-      if (d == 0 || (u >> (shift + 8)) == prefix) atomicAdd(&mine[(u >> shift) & 255u], 1u);
+#pragma unroll 4
+    for (int base = 0; base < sn; base += kEvictThreads) {
+      const int i = base + tid;
+      const uint32_t u = i < sn ? key(i) : 0u;
+      const bool in = i < sn && (d == 0 || (u >> (shift + bits)) == prefix);
+      const uint32_t digit = (u >> shift) & mask;
+      // The first lane's digit is counted once for the warp: equal weights (zeros, as a
+      // rule) would otherwise queue up at one address.
+      const unsigned act = __ballot_sync(0xffffffffu, in);
+      if (act == 0u) continue;
+      const int lead = __ffs(act) - 1;
+      const uint32_t d0 = __shfl_sync(0xffffffffu, digit, lead);
+      const unsigned same = __ballot_sync(0xffffffffu, in && digit == d0);
+      if (lane == lead) atomicAdd(&mine[d0], static_cast<uint32_t>(__popc(same)));
+      else if (in && digit != d0) atomicAdd(&mine[digit], 1u);
     }
     // All CTAs' histograms of this digit are complete, and those of the digit before have
     // been read.
     dev::cluster_sync_all();
-    uint32_t sum = 0;
-    if (tid < 256) {
-      for (int r = 0; r < cs; ++r) sum += ld_cluster_u32(&mine[tid], static_cast<uint32_t>(r));
-      sums[tid] = sum;
-      hist[(d & 1) ^ 1][tid] = 0;
+    // Thread t holds the four digits 2047 - 4 t - e, from the largest down (digits above
+    // the mask are empty).
+    constexpr int PER = kEvictBins / kEvictThreads;
+    static_assert(PER == 4, "one 16-byte load per thread and CTA");
+    const int low = kEvictBins - PER * (tid + 1);
+    uint32_t c[PER] = {0, 0, 0, 0}, own = 0;
+    if (static_cast<uint32_t>(low) <= mask) {
+      uint4 x[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        x[r] = r < cs ? ld_cluster_v4(&mine[low], static_cast<uint32_t>(r)) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+      for (int r = 0; r < 8; ++r) c[0] += x[r].w, c[1] += x[r].z, c[2] += x[r].y, c[3] += x[r].x;
     }
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+      own += c[e];
+      hist[(d & 1) ^ 1][low + e] = 0;
+    }
+    uint32_t inc = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    if (lane == 31) warp_a[warp] = inc;
+    if (tid == 0) pick[0] = mask, pick[1] = 0u;  // left == 0: nothing is wanted
     __syncthreads();
-    // Warp 0: the digit in which the `left`-th largest key lies. Lane l holds digits
-    // 255 - 8 l - e, from the largest down.
-    if (warp == 0) {
-      uint32_t own = 0;
+    uint32_t run = inc - own;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) own += sums[255 - 8 * lane - e];
-      uint32_t inc = own;
+    for (int w = 0; w < kEvictWarps; ++w) run += w < warp ? warp_a[w] : 0u;
+    // The `left`-th largest key lies in one thread's digits.
+    if (run < left && run + own >= left) {
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += v;
-      }
-      uint32_t run = inc - own;
-      const bool here = run < left && inc >= left;
-      if (here) {
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t c = sums[255 - 8 * lane - e];
-          if (run + c >= left) {
-            pick[0] = static_cast<uint32_t>(255 - 8 * lane - e);
-            pick[1] = run;
-            break;
-          }
-          run += c;
+      for (int e = 0; e < PER; ++e) {
+        if (run < left && run + c[e] >= left) {
+          pick[0] = static_cast<uint32_t>(kEvictBins - 1 - PER * tid - e);
+          pick[1] = run;
         }
+        run += c[e];
       }
-      // left == 0: nothing above the largest digit is wanted.
-      if (left == 0 && lane == 0) pick[0] = 255u, pick[1] = 0u;
     }
     __syncthreads();
-    const uint32_t digit = pick[0];
-    // This CTA's keys above the chosen digit (the others' likewise, in their CTAs).
-    if (warp == 0) {
-      uint32_t c = 0;
-      for (uint32_t x = digit + 1 + lane; x < 256; x += 32) c += mine[x];
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
-      above += c;
-      if (d == 3 && lane == 0) {
-        counts[0] = above;
-        counts[1] = mine[digit];
-      }
-    }
     left -= pick[1];
-    prefix = (prefix << 8) | digit;
+    prefix = (prefix << bits) | pick[0];
     __syncthreads();
   }
+  // Keys above and equal to the threshold in each warp's contiguous part.
+  const int part = ((sn + kEvictWarps - 1) / kEvictWarps + 31) & ~31;
+  const int w0 = min(sn, warp * part), w1 = min(sn, w0 + part);
+  uint32_t gt_n = 0, eq_n = 0;
+#pragma unroll 4
+  for (int i = w0 + lane; i < w1; i += 32) {
+    const uint32_t u = key(i);
+    gt_n += u > prefix ? 1u : 0u;
+    eq_n += u == prefix ? 1u : 0u;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    gt_n += __shfl_xor_sync(0xffffffffu, gt_n, o);
+    eq_n += __shfl_xor_sync(0xffffffffu, eq_n, o);
+  }
+  if (lane == 0) warp_a[warp] = gt_n, warp_b[warp] = eq_n;
+  __syncthreads();
+  if (tid == 0) {
+    uint32_t g = 0, q = 0;
+    for (int w = 0; w < kEvictWarps; ++w) g += warp_a[w], q += warp_b[w];
+    counts[0] = g;
+    counts[1] = q;
+  }
   dev::cluster_sync_all();
-  // `left` keys equal to the threshold are kept, the first ones. What the slices before
-  // this one keep:
+  // `left` keys equal to the threshold are kept, the first ones. What the slices, and the
+  // warps' parts, before this one keep:
   uint32_t eq_before = 0, out = 0;
   for (uint32_t r = 0; r < rank; ++r) {
     const uint32_t gt = ld_cluster_u32(&counts[0], r), eq = ld_cluster_u32(&counts[1], r);
     out += gt + min(eq, left - min(left, eq_before));
     eq_before += eq;
   }
-  dev::cluster_sync_all();  // no CTA leaves while its counts may be read
-  for (int base = 0, it = 0; base < sn; base += kEvictThreads, ++it) {
-    const int i = base + tid;
-    const uint32_t u = i < sn ? key(i) : 0u;
-    const bool gt = i < sn && u > prefix, eq = i < sn && u == prefix;
+  for (int w = 0; w < warp; ++w) {
+    out += warp_a[w] + min(warp_b[w], left - min(left, eq_before));
+    eq_before += warp_b[w];
+  }
+  dev::cluster_arrive();  // no CTA leaves while its counts may be read
+  const unsigned below = (1u << lane) - 1u;
+#pragma unroll 4
+  for (int base = w0; base < w1; base += 32) {
+    const int i = base + lane;
+    const uint32_t u = i < w1 ? key(i) : 0u;
+    const bool eq = i < w1 && u == prefix;
     const unsigned eq_b = __ballot_sync(0xffffffffu, eq);
-    if (lane == 0) warp_eq[it & 1][warp] = __popc(eq_b);
-    __syncthreads();
-    // Equal keys in the warps before this one, and in the strip.
-    const uint32_t ew = warp_eq[it & 1][lane];
-    uint32_t e_inc = ew;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t v = __shfl_up_sync(0xffffffffu, e_inc, o);
-      if (lane >= o) e_inc += v;
-    }
-    const uint32_t e_warp = __shfl_sync(0xffffffffu, e_inc - ew, warp);
-    const uint32_t e_all = __shfl_sync(0xffffffffu, e_inc, 31);
-    const uint32_t e_rank = eq_before + e_warp + __popc(eq_b & ((1u << lane) - 1u));
-    const bool take = gt || (eq && e_rank < left);
+    const bool take = (i < w1 && u > prefix) || (eq && eq_before + __popc(eq_b & below) < left);
     const unsigned tk = __ballot_sync(0xffffffffu, take);
-    if (lane == 0) warp_take[it & 1][warp] = __popc(tk);
-    __syncthreads();
-    const uint32_t tw = warp_take[it & 1][lane];
-    uint32_t t_inc = tw;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t v = __shfl_up_sync(0xffffffffu, t_inc, o);
-      if (lane >= o) t_inc += v;
-    }
-    const uint32_t t_warp = __shfl_sync(0xffffffffu, t_inc - tw, warp);
-    const uint32_t t_all = __shfl_sync(0xffffffffu, t_inc, 31);
-    if (take) kept[out + t_warp + __popc(tk & ((1u << lane) - 1u))] = s0 + i;
-    out += t_all;
-    eq_before += e_all;
+    if (take) kept[out + __popc(tk & below)] = s0 + i;
+    out += __popc(tk);
+    eq_before += __popc(eq_b);
   }
   // The recent keys.
   for (int j = static_cast<int>(rank) * kEvictThreads + tid; j < p.recent; j += cs * kEvictThreads)
     kept[want + j] = m + j;
+  __syncwarp();
+  dev::cluster_wait();
 }
 
-// LPR lanes of 16 bytes per row; ROWS rows of one (sequence, head) per lane.
+// LPR lanes of 16 bytes per row; ROWS rows of one (sequence, head) per lane and step.
 template <int LPR, int ROWS>
-__global__ void __launch_bounds__(256) evict_copy_kernel(const EvictParams p, int strips) {
+__global__ void __launch_bounds__(256, 3) evict_copy_kernel(const EvictParams p, int strips, int total) {
   constexpr int PER = 256 / LPR;  // rows at a time
   const int piece = static_cast<int>(threadIdx.x) % LPR, slot = static_cast<int>(threadIdx.x) / LPR;
-  const long long row = blockIdx.x / strips;
-  const int strip = static_cast<int>(blockIdx.x - row * strips);
-  const int b = static_cast<int>(row / p.cache.kv_heads);
-  const int h = static_cast<int>(row - static_cast<long long>(b) * p.cache.kv_heads);
   const int page_mask = (1 << p.cache.page_shift) - 1;
-  dev::grid_dependency_wait();
-  const int j0 = strip * (PER * ROWS) + slot;
-  const int* kept = p.kept + row * p.budget;
-  long long src[ROWS], dst[ROWS];  // element offsets, -1: no row
-  long long wsrc[ROWS], wdst[ROWS];
-#pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    const int j = j0 + i * PER;
-    src[i] = -1;
-    const int t = j < p.budget ? kept[j] : -1;
-    if (t < 0) continue;
-    const int sp = p.page_table[b * p.table_stride + (t >> p.cache.page_shift)];
-    const int dp = p.dst_table[b * p.dst_stride + (j >> p.cache.page_shift)];
-    if (sp < 0 || sp >= p.cache.num_pages || dp < 0 || dp >= p.cache.num_pages) {
-      dev::record_error(dev::kDevErrBadIndex);
-      continue;
-    }
-    src[i] = sp * p.cache.page_stride + (t & page_mask) * p.cache.token_stride + h * p.cache.head_stride;
-    dst[i] = dp * p.cache.page_stride + (j & page_mask) * p.cache.token_stride + h * p.cache.head_stride;
-    wsrc[i] = ((static_cast<long long>(sp) * p.cache.kv_heads + h) << p.cache.page_shift) + (t & page_mask);
-    wdst[i] = ((static_cast<long long>(dp) * p.cache.kv_heads + h) << p.cache.page_shift) + (j & page_mask);
-  }
   const char* k = static_cast<const char*>(p.cache.K) + piece * 16;
   const char* v = static_cast<const char*>(p.cache.V) + piece * 16;
-  uint4 kr[ROWS], vr[ROWS];
-  float w[ROWS];
+  dev::grid_dependency_wait();
+  // Cache slots of a step's rows, source and destination; -1: no row.
+  int src[ROWS], dst[ROWS], next_h = 0;
+  auto look_up = [&](int step) {
+    const int row = step / strips, strip = step - row * strips;
+    const int b = row / p.cache.kv_heads;
+    next_h = row - b * p.cache.kv_heads;
+    const int* kept = p.kept + static_cast<long long>(row) * p.budget;
+    int t[ROWS], sp[ROWS], dp[ROWS];
 #pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    if (src[i] < 0) continue;
-    kr[i] = *reinterpret_cast<const uint4*>(k + src[i] * p.elem);
-    vr[i] = *reinterpret_cast<const uint4*>(v + src[i] * p.elem);
-    w[i] = p.key_weights[wsrc[i]];
-  }
+    for (int i = 0; i < ROWS; ++i) {
+      const int j = strip * (PER * ROWS) + i * PER + slot;
+      t[i] = j < p.budget ? kept[j] : -1;
+      dp[i] = j < p.budget ? p.dst_table[b * p.dst_stride + (j >> p.cache.page_shift)] : 0;
+    }
 #pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    if (src[i] < 0) continue;
-    *reinterpret_cast<uint4*>(const_cast<char*>(k) + dst[i] * p.elem) = kr[i];
-    *reinterpret_cast<uint4*>(const_cast<char*>(v) + dst[i] * p.elem) = vr[i];
-    if (piece == 0) p.key_weights[wdst[i]] = w[i];
+    for (int i = 0; i < ROWS; ++i)
+      sp[i] = t[i] >= 0 ? p.page_table[b * p.table_stride + (t[i] >> p.cache.page_shift)] : -1;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const int j = strip * (PER * ROWS) + i * PER + slot;
+      const bool ok = sp[i] >= 0 && sp[i] < p.cache.num_pages && dp[i] >= 0 && dp[i] < p.cache.num_pages;
+      bad = bad || (t[i] >= 0 && !ok);
+      src[i] = t[i] >= 0 && ok ? (sp[i] << p.cache.page_shift) + (t[i] & page_mask) : -1;
+      dst[i] = (dp[i] << p.cache.page_shift) + (j & page_mask);
+    }
+    if (bad) dev::record_error(dev::kDevErrBadIndex);
+  };
+  const long long page_b = p.cache.page_stride * p.elem, tok_b = p.cache.token_stride * p.elem;
+  int step = static_cast<int>(blockIdx.x);
+  if (step < total) look_up(step);
+  for (; step < total; step += static_cast<int>(gridDim.x)) {
+    const int h = next_h;
+    const long long head = h * p.cache.head_stride * p.elem;
+    uint4 kr[ROWS], vr[ROWS];
+    float w[ROWS];
+    int to[ROWS];
+    // Row h of slot s in the paged weights.
+    auto weight_at = [&](int s) {
+      return ((static_cast<long long>(s >> p.cache.page_shift) * p.cache.kv_heads + h) << p.cache.page_shift) +
+             (s & page_mask);
+    };
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      to[i] = src[i] < 0 ? -1 : dst[i];
+      if (src[i] < 0) continue;
+      const long long off = (src[i] >> p.cache.page_shift) * page_b + (src[i] & page_mask) * tok_b + head;
+      kr[i] = *reinterpret_cast<const uint4*>(k + off);
+      vr[i] = *reinterpret_cast<const uint4*>(v + off);
+      w[i] = p.key_weights[weight_at(src[i])];
+    }
+    if (step + static_cast<int>(gridDim.x) < total) look_up(step + static_cast<int>(gridDim.x));
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      if (to[i] < 0) continue;
+      const long long off = (to[i] >> p.cache.page_shift) * page_b + (to[i] & page_mask) * tok_b + head;
+      *reinterpret_cast<uint4*>(const_cast<char*>(k) + off) = kr[i];
+      *reinterpret_cast<uint4*>(const_cast<char*>(v) + off) = vr[i];
+      if (piece == 0) p.key_weights[weight_at(to[i])] = w[i];
+    }
   }
 }
 
@@ -267,15 +340,17 @@ namespace {
 std::atomic<uint64_t> g_evict_attr{0};
 
 template <int LPR>
-int launch_copy(const kern::EvictParams& p, cudaStream_t stream) {
+int launch_copy(const kern::EvictParams& p, const DeviceInfo& dev, cudaStream_t stream) {
   constexpr int kRows = 4;
   const int per = 256 / LPR * kRows;
   const int strips = (p.budget + per - 1) / per;
-  const long long blocks = static_cast<long long>(p.batch) * p.cache.kv_heads * strips;
-  if (blocks > 0x7fffffffLL) return fail(CLOVE_ERR_UNSUPPORTED, "evict_cache: too many rows");
+  const long long total = static_cast<long long>(p.batch) * p.cache.kv_heads * strips;
+  if (total > 0x7fffffffLL - 65536) return fail(CLOVE_ERR_UNSUPPORTED, "evict_cache: too many rows");
+  const unsigned blocks = static_cast<unsigned>(std::min<long long>(total, 3LL * dev.num_sms));
   cudaLaunchAttribute la[1];
-  cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>(blocks)), 256, 0, stream, la);
-  return check_cuda(cudaLaunchKernelEx(&cfg, kern::evict_copy_kernel<LPR, kRows>, p, strips),
+  cudaLaunchConfig_t cfg = pdl_config(dim3(blocks), 256, 0, stream, la);
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern::evict_copy_kernel<LPR, kRows>, p, strips,
+                                       static_cast<int>(total)),
                     "evict copy launch");
 }
 
@@ -285,14 +360,18 @@ int launch_evict_cache(const kern::EvictParams& p, const DeviceInfo& dev, cudaSt
   constexpr int kSmem = kern::kEvictCached * 4;
   const uint64_t bit = 1ull << (dev.device & 63);
   if ((g_evict_attr.load(std::memory_order_acquire) & bit) == 0) {
-    const int rc = check_cuda(cudaFuncSetAttribute(kern::evict_select_kernel,
-                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem),
-                              "cudaFuncSetAttribute(evict smem)");
+    int rc = check_cuda(cudaFuncSetAttribute(kern::evict_select_kernel<false>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem),
+                        "cudaFuncSetAttribute(evict smem)");
+    if (!rc)
+      rc = check_cuda(cudaFuncSetAttribute(kern::evict_select_kernel<true>,
+                                           cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem),
+                      "cudaFuncSetAttribute(evict smem)");
     if (rc) return rc;
     g_evict_attr.fetch_or(bit, std::memory_order_acq_rel);
   }
   // CTAs per (sequence, head): up to 8 while all of them fit on the GPU at once (two per
-  // SM) and each still has a strip of 1024 keys.
+  // SM) and each still has a strip of 512 keys.
   const long long rows = static_cast<long long>(p.batch) * p.cache.kv_heads;
   int cs = 1;
   while (cs < 8 && rows * cs * 2 <= 2LL * dev.num_sms && p.capacity > cs * kern::kEvictThreads) cs *= 2;
@@ -306,13 +385,16 @@ int launch_evict_cache(const kern::EvictParams& p, const DeviceInfo& dev, cudaSt
   la[1].val.clusterDim.y = 1;
   la[1].val.clusterDim.z = 1;
   cfg.numAttrs = 2;
-  int rc = check_cuda(cudaLaunchKernelEx(&cfg, kern::evict_select_kernel, p, cs), "evict select launch");
+  const int rc = check_cuda(slice > kern::kEvictCached
+                                ? cudaLaunchKernelEx(&cfg, kern::evict_select_kernel<true>, p, cs)
+                                : cudaLaunchKernelEx(&cfg, kern::evict_select_kernel<false>, p, cs),
+                            "evict select launch");
   if (rc) return rc;
   switch (p.row_bytes) {
-    case 64: return launch_copy<4>(p, stream);
-    case 128: return launch_copy<8>(p, stream);
-    case 256: return launch_copy<16>(p, stream);
-    default: return launch_copy<32>(p, stream);
+    case 64: return launch_copy<4>(p, dev, stream);
+    case 128: return launch_copy<8>(p, dev, stream);
+    case 256: return launch_copy<16>(p, dev, stream);
+    default: return launch_copy<32>(p, dev, stream);
   }
 }
 

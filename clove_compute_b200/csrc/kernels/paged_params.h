@@ -22,25 +22,26 @@ struct PagedCache {
   float v_scale;
 };
 
-// qk_norm_rope.cu
+// qk_norm_rope.cu. One kind of row (queries, keys, values) of every token.
+struct RopePart {
+  const void* in;
+  void* out;           // null: not wanted (keys with a cache; values)
+  const void* weight;  // null: no norm
+  long long in_stride, out_stride;
+  int rows;  // per token; 0: none
+  // Filled by the launcher: the kind's first block, log2 of the rows of a token side by
+  // side, blocks per group of tokens.
+  unsigned first;
+  int shift, chunks;
+};
 struct RopeParams {
-  const void* q;
-  const void* k;
-  const void* v;
-  const void* q_weight;
-  const void* k_weight;
+  RopePart part[3];
   const float* table;
   const int* positions;
   const int* slots;  // null: no cache
-  void* q_out;
-  void* k_out;  // may be null with a cache
-  long long q_stride, k_stride, v_stride, q_out_stride, k_out_stride;
-  int tokens, heads, kv_heads;
-  int rows;    // rows per token: heads + kv_heads, with a cache + kv_heads more
-  int chunks;  // ceil(rows / HPT): lanes' tasks per token
-  int table_len, rotary;
-  int interleaved;
+  int tokens, table_len, rotary, interleaved;
   float eps;
+  float k_per_scale, v_per_scale;  // 1 / the cache's scales
   PagedCache cache;
 };
 

@@ -149,7 +149,7 @@ int launch_exp2_poly_probe(const float* x, float* y, int n, cudaStream_t stream)
 
 // ---- paged key-value cache (kernels/qk_norm_rope.cu, paged_attention_*.cu,
 // paged_key_weights.cu, evict_cache.cu)
-// cache_dtype: the cache's (or dtype without one); fills p.chunks.
+// cache_dtype: the cache's (or dtype without one); fills the parts' launch fields.
 int launch_qk_norm_rope(kern::RopeParams& p, int head_dim, int dtype, int cache_dtype,
                         const DeviceInfo& dev, cudaStream_t stream);
 int read_clear_error_rope();

@@ -212,8 +212,8 @@ int clove_qk_norm_rope(const void* Q, const void* K, const void* V, long long q_
     return fail(CLOVE_ERR_INVALID_ARG, "dtype must be CLOVE_DTYPE_F16 or CLOVE_DTYPE_BF16");
   if (head_dim != 64 && head_dim != 128 && head_dim != 256)
     return fail(CLOVE_ERR_UNSUPPORTED, "head_dim %d (64, 128 and 256 are supported)", head_dim);
-  if (rotary_dim <= 0 || rotary_dim % 8 != 0 || rotary_dim > head_dim)
-    return fail(CLOVE_ERR_UNSUPPORTED, "rotary_dim %d must be a multiple of 8 up to head_dim", rotary_dim);
+  if (rotary_dim <= 0 || rotary_dim % 16 != 0 || rotary_dim > head_dim)
+    return fail(CLOVE_ERR_UNSUPPORTED, "rotary_dim %d must be a multiple of 16 up to head_dim", rotary_dim);
   if (table_len <= 0) return fail(CLOVE_ERR_INVALID_ARG, "the rotation table is empty");
   if ((q_weight == nullptr) != (k_weight == nullptr))
     return fail(CLOVE_ERR_INVALID_ARG, "q_weight and k_weight: both or neither");
@@ -248,34 +248,24 @@ int clove_qk_norm_rope(const void* Q, const void* K, const void* V, long long q_
     return fail(CLOVE_ERR_INVALID_ARG, "a token stride is smaller than the token's heads");
   if (q_stride % 8 || k_stride % 8 || (V && v_stride % 8) || q_out_stride % 8 || (K_out && k_out_stride % 8))
     return fail(CLOVE_ERR_UNSUPPORTED, "token strides must be multiples of 8 elements");
-  if (static_cast<long long>(num_heads) + 2LL * num_kv_heads > (1 << 24))
-    return fail(CLOVE_ERR_UNSUPPORTED, "too many heads");
+  if (static_cast<long long>(num_heads) + 2LL * num_kv_heads > 65535)
+    return fail(CLOVE_ERR_UNSUPPORTED, "over 65535 head rows per token");
   DeviceInfo dev;
   const int rc = current_device(&dev);
   if (rc) return rc;
-  p.q = Q;
-  p.k = K;
-  p.v = V;
-  p.q_weight = q_weight;
-  p.k_weight = k_weight;
+  p.part[0] = kern::RopePart{Q, Q_out, q_weight, q_stride, q_out_stride, num_heads, 0u, 0, 0};
+  p.part[1] = kern::RopePart{K, K_out, k_weight, k_stride, k_out_stride, num_kv_heads, 0u, 0, 0};
+  p.part[2] = kern::RopePart{V, nullptr, nullptr, v_stride, 0, cache != nullptr ? num_kv_heads : 0, 0u, 0, 0};
   p.table = rope_table;
   p.positions = positions;
   p.slots = slots;
-  p.q_out = Q_out;
-  p.k_out = K_out;
-  p.q_stride = q_stride;
-  p.k_stride = k_stride;
-  p.v_stride = v_stride;
-  p.q_out_stride = q_out_stride;
-  p.k_out_stride = k_out_stride;
   p.tokens = num_tokens;
-  p.heads = num_heads;
-  p.kv_heads = num_kv_heads;
-  p.rows = num_heads + num_kv_heads * (cache != nullptr ? 2 : 1);
   p.table_len = table_len;
   p.rotary = rotary_dim;
   p.interleaved = interleaved != 0;
   p.eps = eps;
+  p.k_per_scale = cache != nullptr ? 1.f / p.cache.k_scale : 1.f;
+  p.v_per_scale = cache != nullptr ? 1.f / p.cache.v_scale : 1.f;
   return launch_qk_norm_rope(p, head_dim, dtype, cache_dtype, dev, static_cast<cudaStream_t>(stream));
 }
 

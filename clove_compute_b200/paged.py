@@ -152,7 +152,8 @@ def qk_norm_rope(Q, K, rope_table, positions, q_weight=None, k_weight=None, eps:
                  interleaved: bool = False, V=None, cache: PagedCache | None = None, slots=None,
                  Q_out=None, K_out=None, stream=None):
     """Per-head RMS norm of Q [T, heads, D] and K [T, kv_heads, D] (fp16 or bf16; weights
-    [D], or none), rotation by rope_table[positions], and, with a cache, the rotated K and
+    [D], or none), rotation of the first rope_table.shape[1] (a multiple of 16) elements by
+    rope_table[positions], and, with a cache, the rotated K and
     V rows stored at its `slots`. Rows may be column blocks of a fused projection. Returns
     (Q_out, K_out); with a cache K_out is None unless it was given. Q_out may be Q and
     K_out K. Negative positions mark padding tokens (nothing written), negative slots

@@ -189,7 +189,7 @@ typedef struct {
  * token t at t * *_stride elements (multiples of 8: column blocks of a fused projection).
  * y = x / sqrt(mean(x^2) + eps) * weight per head, weights [D] of the same type (both
  * NULL: no norm); then pair (i, i + rotary_dim/2), or (2i, 2i + 1) when interleaved, of
- * the first rotary_dim elements is turned by row positions[t] of rope_table [table_len,
+ * the first rotary_dim (a multiple of 16) elements is turned by row positions[t] of rope_table [table_len,
  * rotary_dim] fp32: rotary_dim/2 cosines, then as many sines. fp32, rounded once.
  * Q_out (may be Q with the same stride) gets the queries, K_out (may be K, or NULL with a
  * cache) the keys; with a cache, K and V rows also go to slot slots[t] (a negative slot:

@@ -63,7 +63,7 @@ def test_cache_descriptions_refused(clove_lib, bad, code):
 
 @pytest.mark.parametrize("kw,code", [
     (dict(T=-1), 1), (dict(H=0), 1), (dict(Hkv=0), 1), (dict(dtype=2), 1), (dict(D=96), 2),
-    (dict(R=0), 2), (dict(R=20), 2), (dict(R=136), 2), (dict(tl=0), 1), (dict(qw=A), 1), (dict(kw=A), 1),
+    (dict(R=0), 2), (dict(R=24), 2), (dict(R=144), 2), (dict(tl=0), 1), (dict(qw=A), 1), (dict(kw=A), 1),
     (dict(eps=-1.0), 1), (dict(eps=float("nan")), 1), (dict(V=A), 1), (dict(slots=A), 1), (dict(Q=None), 1),
     (dict(Ko=None), 1), (dict(pos=None), 1), (dict(table=None), 1), (dict(Q=A + 2), 2), (dict(table=A + 4), 2),
     (dict(pos=A + 2), 1), (dict(qs=255), 1), (dict(qs=260), 2), (dict(kos=8), 1),

@@ -341,20 +341,27 @@ def _close(got, want, mag, dtype, scale=1.0):
     (7, 8, 2, 128, 128, BF16, E4M3, True, True, "bhsd"),
     (33, 5, 1, 128, 64, F16, E4M3, False, True, "bshd"),
     (65, 4, 4, 64, 64, F16, F16, True, False, "bhsd"),
-    (65, 4, 2, 64, 8, BF16, BF16, False, True, "bshd"),
+    (65, 4, 2, 64, 16, BF16, BF16, False, True, "bshd"),
     (130, 3, 1, 256, 256, F16, F16, False, True, "bshd"),
-    (17, 2, 2, 256, 40, BF16, E4M3, True, True, "bhsd"),
-    (9, 12, 3, 128, 120, F16, None, True, True, "bshd"),
+    (17, 2, 2, 256, 48, BF16, E4M3, True, True, "bhsd"),
+    (9, 12, 3, 128, 112, F16, None, True, True, "bshd"),
     (9, 12, 3, 128, 128, F16, None, False, False, "bshd"),
     (3001, 32, 8, 128, 128, F16, F16, False, True, "bshd"),   # four rows per lane
     (6007, 7, 1, 64, 32, BF16, E4M3, True, True, "bhsd"),
     (4099, 6, 2, 256, 256, BF16, None, False, True, "bshd"),
+    (333, 96, 16, 128, 128, F16, F16, False, True, "bshd"),    # a token's rows in two pieces
+    (700, 100, 33, 256, 192, BF16, E4M3, True, True, "bhsd"),  # in six
 ])
-def test_norm_rope_matches_plain(clove_lib, cuda, T, H, Hkv, D, R, dtype, cache, interleaved, norm, layout):
+@pytest.mark.parametrize("path", [0, 1, 2])  # automatic, the streaming kernel, the direct one
+def test_norm_rope_matches_plain(clove_lib, cuda, T, H, Hkv, D, R, dtype, cache, interleaved, norm, layout, path):
     args, V, c, slots, (yq, mq), (yk, mk) = _norm_rope_case(clove_lib, T, H, Hkv, D, R, dtype, cache, interleaved,
                                                             norm, layout, seed=T + D)
-    q, k = clove_lib.qk_norm_rope(**args, **(dict(V=V, cache=c, slots=slots) if c else {}))
-    torch.cuda.synchronize()
+    clove_lib.set_dispatch_override(path)
+    try:
+        q, k = clove_lib.qk_norm_rope(**args, **(dict(V=V, cache=c, slots=slots) if c else {}))
+        torch.cuda.synchronize()
+    finally:
+        clove_lib.set_dispatch_override(0)
     assert clove_lib.device_error() == 0
     _close(q, yq, mq, dtype)
     if c is None:
@@ -372,9 +379,18 @@ def test_norm_rope_matches_plain(clove_lib, cuda, T, H, Hkv, D, R, dtype, cache,
         assert torch.all(raw[rest].contiguous().view(cache).float() == 5.0)  # other slots stay
 
 
-def test_norm_rope_padding_slots_and_bad_indices(clove_lib, cuda):
+@pytest.mark.parametrize("path", [1, 2])
+def test_norm_rope_padding_slots_and_bad_indices(clove_lib, cuda, path):
     """Padding tokens and tokens without a slot leave everything as it was; positions and
     slots outside their range are reported and not followed."""
+    clove_lib.set_dispatch_override(path)
+    try:
+        _padding_slots_and_bad_indices(clove_lib)
+    finally:
+        clove_lib.set_dispatch_override(0)
+
+
+def _padding_slots_and_bad_indices(clove_lib):
     T, H, Hkv, D = 12, 4, 2, 128
     args, V, c, slots, (yq, mq), (yk, mk) = _norm_rope_case(clove_lib, T, H, Hkv, D, D, F16, F16, False, True, "bshd", 3)
     args["positions"][2] = -1
