@@ -23,11 +23,11 @@
 namespace clove {
 namespace kern {
 
-constexpr int kEvictThreads = 512;
+constexpr int kEvictThreads = 1024;
 constexpr int kEvictWarps = kEvictThreads / 32;
-// Keys of a slice held in shared memory (96 KB: two CTAs per SM); a longer slice reads the
+// Keys of a slice held in shared memory (160 KB: one CTA per SM); a longer slice reads the
 // rest again from memory in every pass.
-constexpr int kEvictCached = 24576;
+constexpr int kEvictCached = 40960;
 constexpr int kEvictBins = 2048;
 
 // Larger weight <=> larger integer; -0 equals 0; every NaN above everything.
@@ -37,13 +37,10 @@ __device__ __forceinline__ uint32_t weight_order(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-__device__ __forceinline__ uint4 ld_cluster_v4(const uint32_t* p, uint32_t rank) {
-  uint4 v;
+__device__ __forceinline__ uint2 ld_cluster_v2(const uint32_t* p, uint32_t rank) {
+  uint2 v;
   const uint32_t a = dev::map_shared_to_rank(dev::smem_u32(p), rank);
-  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(a)
-               : "memory");
+  asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
   return v;
 }
 __device__ __forceinline__ uint32_t ld_cluster_u32(const uint32_t* p, uint32_t rank) {
@@ -55,7 +52,7 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(const uint32_t* p, uint32_t r
 
 // LONG: slices may exceed kEvictCached keys.
 template <bool LONG>
-__global__ void __launch_bounds__(kEvictThreads, 2) evict_select_kernel(const EvictParams p, int cs) {
+__global__ void __launch_bounds__(kEvictThreads, 1) evict_select_kernel(const EvictParams p, int cs) {
   extern __shared__ uint32_t cached[];
   __shared__ __align__(16) uint32_t hist[2][kEvictBins];
   __shared__ uint32_t counts[2];  // this CTA's keys above the threshold, and equal to it
@@ -85,47 +82,53 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_select_kernel(const Ev
   const int m = n - p.recent, want = p.budget - p.recent;
   const int per = (m + cs - 1) / cs;
   const int s0 = min(m, static_cast<int>(rank) * per), sn = min(m, s0 + per) - s0;
-  // Weights of N keys of the slice, kEvictThreads apart, looked up and then read side by
-  // side (no branch between the loads; a bad page counts as weight 0).
+  // Weights of keys of the slice, looked up for sixteen keys at a time before any of them is
+  // read: first all pages (into the keys' places), then all weights. The loads are
+  // unconditional (index and page clamped, the result dropped), so that none waits for
+  // another; a bad page counts as weight 0.
   bool bad = false;
-  auto load = [&](int i0, auto& u) {
-    constexpr int N = sizeof(u) / 4;
-    int pg[N];
-    float w[N];
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const int i = i0 + k * kEvictThreads;
-      pg[k] = i < sn ? p.page_table[b * p.table_stride + ((s0 + i) >> p.cache.page_shift)] : 0;
-    }
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const int i = i0 + k * kEvictThreads;
-      const bool ok = pg[k] >= 0 && pg[k] < p.cache.num_pages;
-      bad = bad || !ok;
-      w[k] = 0.f;
-      if (ok && i < sn)
-        w[k] = p.key_weights[((static_cast<long long>(pg[k]) * p.cache.kv_heads + h) << p.cache.page_shift) +
-                             ((s0 + i) & page_mask)];
-    }
-#pragma unroll
-    for (int k = 0; k < N; ++k) u[k] = weight_order(w[k]);
+  auto page_at = [&](int i) { return p.page_table[b * p.table_stride + ((s0 + i) >> p.cache.page_shift)]; };
+  auto good = [&](int pg) { return pg >= 0 && pg < p.cache.num_pages; };
+  auto weight_at = [&](int i, int pg) {
+    return p.key_weights[((static_cast<long long>(good(pg) ? pg : 0) * p.cache.kv_heads + h)
+                          << p.cache.page_shift) +
+                         ((s0 + i) & page_mask)];
   };
   for (int i = tid; i < kEvictBins; i += kEvictThreads) hist[0][i] = 0;
   const int in_smem = LONG ? min(sn, kEvictCached) : sn;
-  for (int i0 = tid; i0 < in_smem; i0 += 8 * kEvictThreads) {
-    uint32_t u[8];
-    load(i0, u);
+  constexpr int DEEP = 16;
+  for (int i0 = tid; i0 < in_smem; i0 += DEEP * kEvictThreads) {
+    int pg[DEEP];
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (i0 + k * kEvictThreads < in_smem) cached[i0 + k * kEvictThreads] = u[k];
+    for (int k = 0; k < DEEP; ++k) pg[k] = page_at(min(i0 + k * kEvictThreads, in_smem - 1));
+#pragma unroll
+    for (int k = 0; k < DEEP; ++k)
+      if (i0 + k * kEvictThreads < in_smem) cached[i0 + k * kEvictThreads] = static_cast<uint32_t>(pg[k]);
+  }
+  for (int i0 = tid; i0 < in_smem; i0 += DEEP * kEvictThreads) {
+    int pg[DEEP];
+    float w[DEEP];
+#pragma unroll
+    for (int k = 0; k < DEEP; ++k) {  // (only this thread's own places hold pages still)
+      const int i = i0 + k * kEvictThreads;
+      pg[k] = static_cast<int>(cached[i < in_smem ? i : i0]);
+    }
+#pragma unroll
+    for (int k = 0; k < DEEP; ++k) w[k] = weight_at(min(i0 + k * kEvictThreads, in_smem - 1), pg[k]);
+#pragma unroll
+    for (int k = 0; k < DEEP; ++k) {
+      if (i0 + k * kEvictThreads < in_smem) cached[i0 + k * kEvictThreads] = weight_order(good(pg[k]) ? w[k] : 0.f);
+      bad = bad || !good(pg[k]);
+    }
   }
   if (bad) dev::record_error(dev::kDevErrBadIndex);
   __syncthreads();
   auto key = [&](int i) {
     if (!LONG || i < in_smem) return cached[i];
-    uint32_t u[1];
-    load(i, u);
-    return u[0];
+    const int pg = page_at(i);
+    const float w = weight_at(i, pg);
+    if (!good(pg)) dev::record_error(dev::kDevErrBadIndex);
+    return weight_order(good(pg) ? w : 0.f);
   };
 
   uint32_t prefix = 0;  // digits chosen so far
@@ -153,25 +156,22 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_select_kernel(const Ev
     // All CTAs' histograms of this digit are complete, and those of the digit before have
     // been read.
     dev::cluster_sync_all();
-    // Thread t holds the four digits 2047 - 4 t - e, from the largest down (digits above
-    // the mask are empty).
+    // Thread t holds the digits 2047 - 2 t and 2046 - 2 t: from the largest down (digits
+    // above the mask are empty).
     constexpr int PER = kEvictBins / kEvictThreads;
-    static_assert(PER == 4, "one 16-byte load per thread and CTA");
+    static_assert(PER == 2, "one 8-byte load per thread and CTA");
     const int low = kEvictBins - PER * (tid + 1);
-    uint32_t c[PER] = {0, 0, 0, 0}, own = 0;
+    uint32_t c[PER] = {0, 0};
     if (static_cast<uint32_t>(low) <= mask) {
-      uint4 x[8];
+      uint2 x[8];
 #pragma unroll
       for (int r = 0; r < 8; ++r)
-        x[r] = r < cs ? ld_cluster_v4(&mine[low], static_cast<uint32_t>(r)) : make_uint4(0u, 0u, 0u, 0u);
+        x[r] = r < cs ? ld_cluster_v2(&mine[low], static_cast<uint32_t>(r)) : make_uint2(0u, 0u);
 #pragma unroll
-      for (int r = 0; r < 8; ++r) c[0] += x[r].w, c[1] += x[r].z, c[2] += x[r].y, c[3] += x[r].x;
+      for (int r = 0; r < 8; ++r) c[0] += x[r].y, c[1] += x[r].x;
     }
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      own += c[e];
-      hist[(d & 1) ^ 1][low + e] = 0;
-    }
+    const uint32_t own = c[0] + c[1];
+    hist[(d & 1) ^ 1][low] = hist[(d & 1) ^ 1][low + 1] = 0;
     uint32_t inc = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -182,8 +182,12 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_select_kernel(const Ev
     if (tid == 0) pick[0] = mask, pick[1] = 0u;  // left == 0: nothing is wanted
     __syncthreads();
     uint32_t run = inc - own;
+    {  // the warps before this one: one lane each
+      uint32_t v = lane < warp ? warp_a[lane] : 0u;
 #pragma unroll
-    for (int w = 0; w < kEvictWarps; ++w) run += w < warp ? warp_a[w] : 0u;
+      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      run += v;
+    }
     // The `left`-th largest key lies in one thread's digits.
     if (run < left && run + own >= left) {
 #pragma unroll
@@ -217,11 +221,14 @@ __global__ void __launch_bounds__(kEvictThreads, 2) evict_select_kernel(const Ev
   }
   if (lane == 0) warp_a[warp] = gt_n, warp_b[warp] = eq_n;
   __syncthreads();
-  if (tid == 0) {
-    uint32_t g = 0, q = 0;
-    for (int w = 0; w < kEvictWarps; ++w) g += warp_a[w], q += warp_b[w];
-    counts[0] = g;
-    counts[1] = q;
+  if (warp == 0) {
+    uint32_t g = warp_a[lane], q = warp_b[lane];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      g += __shfl_xor_sync(0xffffffffu, g, o);
+      q += __shfl_xor_sync(0xffffffffu, q, o);
+    }
+    if (lane == 0) counts[0] = g, counts[1] = q;
   }
   dev::cluster_sync_all();
   // `left` keys equal to the threshold are kept, the first ones. What the slices, and the
@@ -273,16 +280,20 @@ __global__ void __launch_bounds__(256, 3) evict_copy_kernel(const EvictParams p,
     const int b = row / p.cache.kv_heads;
     next_h = row - b * p.cache.kv_heads;
     const int* kept = p.kept + static_cast<long long>(row) * p.budget;
+    // (Unconditional loads at clamped places: none waits for a branch on another.)
     int t[ROWS], sp[ROWS], dp[ROWS];
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
-      const int j = strip * (PER * ROWS) + i * PER + slot;
-      t[i] = j < p.budget ? kept[j] : -1;
-      dp[i] = j < p.budget ? p.dst_table[b * p.dst_stride + (j >> p.cache.page_shift)] : 0;
+      const int j = min(strip * (PER * ROWS) + i * PER + slot, p.budget - 1);
+      t[i] = kept[j];
+      dp[i] = p.dst_table[b * p.dst_stride + (j >> p.cache.page_shift)];
     }
 #pragma unroll
     for (int i = 0; i < ROWS; ++i)
-      sp[i] = t[i] >= 0 ? p.page_table[b * p.table_stride + (t[i] >> p.cache.page_shift)] : -1;
+      sp[i] = p.page_table[b * p.table_stride + (max(t[i], 0) >> p.cache.page_shift)];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i)
+      if (strip * (PER * ROWS) + i * PER + slot >= p.budget) t[i] = -1;
     bool bad = false;
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
@@ -370,11 +381,11 @@ int launch_evict_cache(const kern::EvictParams& p, const DeviceInfo& dev, cudaSt
     if (rc) return rc;
     g_evict_attr.fetch_or(bit, std::memory_order_acq_rel);
   }
-  // CTAs per (sequence, head): up to 8 while all of them fit on the GPU at once (two per
-  // SM) and each still has a strip of 512 keys.
+  // CTAs per (sequence, head): up to 8 while all of them fit on the GPU at once (one per
+  // SM) and each still has a strip of 1024 keys.
   const long long rows = static_cast<long long>(p.batch) * p.cache.kv_heads;
   int cs = 1;
-  while (cs < 8 && rows * cs * 2 <= 2LL * dev.num_sms && p.capacity > cs * kern::kEvictThreads) cs *= 2;
+  while (cs < 8 && rows * cs * 2 <= dev.num_sms && p.capacity > cs * kern::kEvictThreads) cs *= 2;
   if (rows * cs > 0x7fffffffLL) return fail(CLOVE_ERR_UNSUPPORTED, "evict_cache: batch x heads exceeds 2^31");
   const int slice = (p.capacity + cs - 1) / cs;
   cudaLaunchAttribute la[2];
@@ -389,7 +400,7 @@ int launch_evict_cache(const kern::EvictParams& p, const DeviceInfo& dev, cudaSt
                                 ? cudaLaunchKernelEx(&cfg, kern::evict_select_kernel<true>, p, cs)
                                 : cudaLaunchKernelEx(&cfg, kern::evict_select_kernel<false>, p, cs),
                             "evict select launch");
-  if (rc) return rc;
+  if (rc || p.capacity == 0) return rc;
   switch (p.row_bytes) {
     case 64: return launch_copy<4>(p, dev, stream);
     case 128: return launch_copy<8>(p, dev, stream);
