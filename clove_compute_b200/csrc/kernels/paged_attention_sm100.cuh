@@ -38,7 +38,7 @@
 namespace clove {
 namespace kern {
 
-constexpr int kPagedWarps = kPagedTile / 16;
+constexpr int kPagedWarps = 4;
 
 template <bool F8, int D, int NT>
 struct PagedShape {
@@ -46,7 +46,11 @@ struct PagedShape {
   static constexpr int HEADS = 8 * NT;             // query heads per item
   static constexpr int ROWB = D * (F8 ? 1 : 2);    // bytes of a K (or V) row
   static constexpr int CPR = ROWB / 16;            // 16-byte pieces per row
-  static constexpr int CHUNK = 16 * ROWB;          // bytes of a warp's K (or V) chunk
+  // Groups of 16 keys per warp and step: two where rows are short, so that a step's fixed
+  // cost (cursors, votes, waits) is paid for 8 KB of keys and values at least.
+  static constexpr int M = ROWB <= 128 ? 2 : 1;
+  static constexpr int TILE = kPagedWarps * 16 * M;  // keys per CTA step
+  static constexpr int CHUNK = 16 * M * ROWB;        // bytes of a warp's K (or V) chunk
   // 24 KB of ring per warp where that holds three chunks (two CTAs per SM), else three
   // chunks (head_dim 256 in 16 bits: one CTA per SM).
   static constexpr int STAGES = 24576 / (2 * CHUNK) >= 8 ? 8
@@ -100,10 +104,14 @@ struct Pair<__nv_bfloat16> {
   }
 };
 
-// Two e4m3 values as two fp16 values (exact).
-__device__ __forceinline__ uint32_t e4m3_to_half2(uint16_t v) {
-  const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2(v, __NV_E4M3);
-  return static_cast<uint32_t>(r.x) | (static_cast<uint32_t>(r.y) << 16);
+// Four e4m3 values as fp16 (exact): the two lower ones in lo, the others in hi.
+__device__ __forceinline__ void e4m3_to_half(uint32_t v, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\t"
+      "mov.b32 {a, b}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, a;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(v));
 }
 
 __device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
@@ -141,6 +149,7 @@ struct PagedCursor {
   int b, h, block, tile;
   PagedSpan s;
 };
+template <int TILE>
 __device__ __forceinline__ void paged_next_item(const PagedAttnParams& p, PagedCursor& c) {
   c.tile = 0;
   if (++c.block < p.blocks) return;
@@ -153,7 +162,7 @@ __device__ __forceinline__ void paged_next_item(const PagedAttnParams& p, PagedC
       c.s = PagedSpan{0, 0, 0, 0};
       return;
     }
-    c.s = paged_span(p, c.b);
+    c.s = paged_span<TILE>(p, c.b);
   } while (c.s.tiles == 0);
 }
 
@@ -170,15 +179,17 @@ __device__ __forceinline__ int warp_scan(int v) {
 
 // Tiles of the sequences [l R, (l+1) R) of lane l, R = per_lane, times items per sequence.
 // (The host has checked that all tiles together stay below 2^31.)
+template <int TILE>
 __device__ __forceinline__ int paged_lane_tiles(const PagedAttnParams& p, int hh_n, int per_lane) {
   const int b0 = static_cast<int>(dev::lane_idx()) * per_lane, b1 = min(p.batch, b0 + per_lane);
   int sum = 0;
-  for (int b = b0; b < b1; ++b) sum += paged_span(p, b).tiles;
+  for (int b = b0; b < b1; ++b) sum += paged_span<TILE>(p, b).tiles;
   return sum * hh_n;
 }
 
 // The (warp-uniform) cursor of tile `at`; own, upto: this lane's tiles and their inclusive
 // sum. The lane that holds the tile names 32 R sequences, which are scanned in strips.
+template <int TILE>
 __device__ __forceinline__ PagedCursor paged_find(const PagedAttnParams& p, int hh_n, int per_lane,
                                                   int own, int upto, int at) {
   const int lane = static_cast<int>(dev::lane_idx());
@@ -189,7 +200,7 @@ __device__ __forceinline__ PagedCursor paged_find(const PagedAttnParams& p, int 
   if (per_lane > 1) {
     const int b_end = min(p.batch, (owner + 1) * per_lane);
     for (int b0 = owner * per_lane; b0 < b_end; b0 += 32) {
-      const int t = b0 + lane < b_end ? paged_span(p, b0 + lane).tiles * hh_n : 0;
+      const int t = b0 + lane < b_end ? paged_span<TILE>(p, b0 + lane).tiles * hh_n : 0;
       const int inc = warp_scan(t);
       const unsigned hit = __ballot_sync(0xffffffffu, before + inc > at);
       if (hit) {
@@ -203,7 +214,7 @@ __device__ __forceinline__ PagedCursor paged_find(const PagedAttnParams& p, int 
   }
   PagedCursor c;
   c.b = b;
-  c.s = paged_span(p, b);
+  c.s = paged_span<TILE>(p, b);
   const int hh = (at - before) / c.s.tiles;
   c.tile = at - before - hh * c.s.tiles;
   c.h = hh / p.blocks;
@@ -290,7 +301,7 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
   // e4m3 elements (and their queries) are multiplied as fp16, whatever the query type.
   using MT = typename std::conditional<F8, __half, T>::type;
   using P2 = Pair<MT>;
-  constexpr int ROWB = S::ROWB, CPR = S::CPR, KK = D / 16;
+  constexpr int ROWB = S::ROWB, CPR = S::CPR, KK = D / 16, M = S::M;
   extern __shared__ __align__(1024) uint8_t smem[];
   float* merge = reinterpret_cast<float*>(smem + kPagedWarps * S::RING);
   float* sm_m = merge + S::MERGE / 4;         // [warp][HEADS]
@@ -319,7 +330,7 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
   }
 
   const int per_lane = (p.batch + 31) / 32;
-  const int own = paged_lane_tiles(p, hh_n, per_lane), upto = warp_scan(own);
+  const int own = paged_lane_tiles<S::TILE>(p, hh_n, per_lane), upto = warp_scan(own);
   const int total = __shfl_sync(0xffffffffu, upto, 31);
   const int workers = min(static_cast<int>(gridDim.x), total);
   if (cta >= workers) return;
@@ -327,19 +338,14 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
   const int share = total / workers, more = total - share * workers;
   const int n_tiles = share + (cta < more ? 1 : 0);
   const int t_begin = cta * share + min(cta, more);
-  PagedCursor cur = paged_find(p, hh_n, per_lane, own, upto, t_begin);
+  PagedCursor cur = paged_find<S::TILE>(p, hh_n, per_lane, own, upto, t_begin);
   PagedCursor ld = cur;  // the loads' place
   int ld_left = n_tiles;
   const int page_mask = (1 << p.cache.page_shift) - 1;
   const bool whole_pages = p.cache.page_shift >= 4;  // a 16-key chunk lies in one page
 
-  auto chunk_key = [&](const PagedCursor& c) { return c.s.base + c.tile * kPagedTile + warp * 16; };
-  auto page_of = [&](int b, int key) {
-    const int pg = p.page_table[b * p.table_stride + (key >> p.cache.page_shift)];
-    if (pg >= 0 && pg < p.cache.num_pages) return pg;
-    dev::record_error(dev::kDevErrBadIndex);
-    return -1;
-  };
+  auto chunk_key = [&](const PagedCursor& c) { return c.s.base + c.tile * S::TILE + warp * (16 * M); };
+  auto good_page = [&](int pg) { return pg >= 0 && pg < p.cache.num_pages; };
   // Byte strides, and this lane's part of the addresses: a chunk is loaded RPI rows at a
   // time, CPR lanes per row; 16-byte piece c of row r lies at piece c ^ swizzle(r).
   constexpr int EB = F8 ? 1 : 2, RPI = 32 / CPR;
@@ -348,14 +354,20 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
   const int ld_row = lane / CPR, piece = lane % CPR;
   const uint8_t* ld_base = static_cast<const uint8_t*>(p.cache.K) + ld_row * tok_b + piece * 16;
   const uint32_t ld_dst = ring + ld_row * ROWB + ((piece ^ S::swizzle(ld_row)) << 4);
-  // Pages of this warp's chunks, where a chunk lies in one page: lane i holds that of tile
-  // win_tile + i of the item that is being loaded; the next 32, and those of the next item,
-  // are read well before they are needed.
+  // Pages of this warp's chunks, where 16 keys lie in one page: lane i holds that of group
+  // i % M of tile win_tile + i / M of the item that is being loaded; the next 32, and those
+  // of the next item, are read well before they are needed. -1: no keys, or a bad page.
+  constexpr int WTILES = 32 / M;
   PagedCursor nx;
   int win = -1, win_tile = 0, win_more = -1, win_next = -1;
   auto window = [&](const PagedCursor& c, int tile) {
-    const int key = c.s.base + (tile + lane) * kPagedTile + warp * 16;
-    return tile + lane < c.s.tiles && key < c.s.len ? page_of(c.b, key) : -1;
+    tile += lane / M;
+    const int key = c.s.base + tile * S::TILE + warp * (16 * M) + lane % M * 16;
+    if (tile >= c.s.tiles || key >= c.s.len) return -1;
+    const int pg = p.page_table[c.b * p.table_stride + (key >> p.cache.page_shift)];
+    if (good_page(pg)) return pg;
+    dev::record_error(dev::kDevErrBadIndex);
+    return -1;
   };
   const uint8_t* ld_src = nullptr;  // this lane's address in row 0 of page 0 for the item's head
   auto enter = [&]() {  // `ld` has come to an item; its window is in win
@@ -363,7 +375,7 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
     ld_src = ld_base + ld.h * p.cache.head_stride * EB;
     if (ld_left > ld.s.tiles - ld.tile) {
       nx = ld;
-      paged_next_item(p, nx);
+      paged_next_item<S::TILE>(p, nx);
       if (whole_pages) win_next = window(nx, 0);
     }
   };
@@ -371,31 +383,54 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
     if (ld_left > 0) {
       const int key = chunk_key(ld);
       const int at = ld.tile - win_tile;
-      const int page = __shfl_sync(0xffffffffu, win, at & 31);
+      int page[M];
+#pragma unroll
+      for (int g = 0; g < M; ++g) page[g] = __shfl_sync(0xffffffffu, win, (at * M + g) & 31);
       if (key < ld.s.len) {
         const uint32_t dst = ld_dst + stage * 2 * S::CHUNK;
-        const uint8_t* src = ld_src;
-        if (whole_pages && page >= 0 && key >= ld.s.first && key + 16 <= ld.s.len) {
-          src += page * p.cache.page_stride * EB + (key & page_mask) * tok_b;
+        bool plain = whole_pages && key >= ld.s.first && key + 16 * M <= ld.s.len;
 #pragma unroll
-          for (int i = 0; i < 16 / RPI; ++i) {
-            // swizzle(ld_row + i RPI) = swizzle(ld_row) ^ swizzle(i RPI): ld_row < RPI.
-            const uint32_t d = (dst ^ (S::swizzle(i * RPI) << 4)) + i * RPI * ROWB;
-            cp_async_16(d, src, 16u);
-            cp_async_16(d + S::CHUNK, src + v_minus_k, 16u);
-            src += RPI * tok_b;
+        for (int g = 0; g < M; ++g) plain = plain && page[g] >= 0;
+        if (plain) {
+#pragma unroll
+          for (int g = 0; g < M; ++g) {
+            const uint8_t* src =
+                ld_src + page[g] * p.cache.page_stride * EB + ((key + 16 * g) & page_mask) * tok_b;
+#pragma unroll
+            for (int i = g * 16 / RPI; i < (g + 1) * 16 / RPI; ++i) {
+              // swizzle(ld_row + i RPI) = swizzle(ld_row) ^ swizzle(i RPI): ld_row < RPI.
+              const uint32_t d = (dst ^ (S::swizzle(i * RPI) << 4)) + i * RPI * ROWB;
+              cp_async_16(d, src, 16u);
+              cp_async_16(d + S::CHUNK, src + v_minus_k, 16u);
+              src += RPI * tok_b;
+            }
           }
         } else {
-          for (int i = 0; i < 16 / RPI; ++i) {
+          // Keys outside the sequence, bad pages, or pages of less than 16 keys: row by row.
+          constexpr int N = 16 * M / RPI;
+          int pg[N];
+          bool bad = false;
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
             const int t = key + ld_row + i * RPI;
-            int pg = -1;
-            if (t >= ld.s.first && t < ld.s.len) pg = whole_pages ? page : page_of(ld.b, t);
+            pg[i] = page[i * RPI / 16];
+            if (!whole_pages)  // (a clamped key: the loads do not wait for one another)
+              pg[i] = p.page_table[ld.b * p.table_stride +
+                                   (max(ld.s.first, min(t, ld.s.len - 1)) >> p.cache.page_shift)];
+          }
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            const int t = key + ld_row + i * RPI;
+            bool ok = t >= ld.s.first && t < ld.s.len;
+            bad = bad || (!whole_pages && ok && !good_page(pg[i]));
+            ok = ok && good_page(pg[i]);
             const uint32_t d = (dst ^ (S::swizzle(i * RPI) << 4)) + i * RPI * ROWB;
             const uint8_t* from =
-                pg < 0 ? src : src + pg * p.cache.page_stride * EB + ((t & page_mask) - ld_row) * tok_b;
-            cp_async_16(d, from, pg < 0 ? 0u : 16u);
-            cp_async_16(d + S::CHUNK, from + v_minus_k, pg < 0 ? 0u : 16u);
+                ok ? ld_src + pg[i] * p.cache.page_stride * EB + ((t & page_mask) - ld_row) * tok_b : ld_src;
+            cp_async_16(d, from, ok ? 16u : 0u);
+            cp_async_16(d + S::CHUNK, from + v_minus_k, ok ? 16u : 0u);
           }
+          if (bad) dev::record_error(dev::kDevErrBadIndex);
         }
       }
       --ld_left;
@@ -406,8 +441,8 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
           enter();
         }
       } else if (whole_pages) {
-        if (at == 15) win_more = window(ld, win_tile + 32);
-        if (at == 31) win = win_more, win_tile += 32;
+        if (at == WTILES / 2 - 1) win_more = window(ld, win_tile + WTILES);
+        if (at == WTILES - 1) win = win_more, win_tile += WTILES;
       }
     }
     cp_async_commit();
@@ -506,72 +541,89 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
     const int key = chunk_key(cur);
     if (key < cur.s.len) {
       const uint32_t ks = ring + stage * 2 * S::CHUNK, vs = ks + S::CHUNK;
-      float sc[NT][4];
+      float sc[M][NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int g = 0; g < M; ++g)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[nt][e] = 0.f;
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[g][nt][e] = 0.f;
       // S^T: rows = keys, columns = heads.
 #pragma unroll
-      for (int c = 0; c < CPR; c += 2) {
-        uint32_t a[4];
-        ldsm_x4(a, (ks + k_lane) ^ (c << 4));
-        if (!F8) {
+      for (int c = 0; c < CPR; c += 2)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) P2::mma(sc[nt], a, qf[nt][c / 2][0], qf[nt][c / 2][1]);
-        } else {
-          // A lane holds four consecutive elements of a row: the first two stand in for
-          // k = 2c, 2c+1 and the others for k = 2c+8, 2c+9, in Q's fragments alike.
+        for (int g = 0; g < M; ++g) {
+          uint32_t a[4];
+          ldsm_x4(a, ((ks + k_lane) ^ (c << 4)) + g * 16 * ROWB);
+          if constexpr (!F8) {
 #pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            uint32_t x[4];
-            x[0] = e4m3_to_half2(static_cast<uint16_t>(a[2 * w]));
-            x[1] = e4m3_to_half2(static_cast<uint16_t>(a[2 * w + 1]));
-            x[2] = e4m3_to_half2(static_cast<uint16_t>(a[2 * w] >> 16));
-            x[3] = e4m3_to_half2(static_cast<uint16_t>(a[2 * w + 1] >> 16));
+            for (int nt = 0; nt < NT; ++nt) P2::mma(sc[g][nt], a, qf[nt][c / 2][0], qf[nt][c / 2][1]);
+          } else {
+            // A lane holds four consecutive elements of a row: the first two stand in for
+            // k = 2c, 2c+1 and the others for k = 2c+8, 2c+9, in Q's fragments alike.
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) P2::mma(sc[nt], x, qf[nt][c + w][0], qf[nt][c + w][1]);
+            for (int w = 0; w < 2; ++w) {
+              uint32_t x[4];
+              e4m3_to_half(a[2 * w], x[0], x[2]);
+              e4m3_to_half(a[2 * w + 1], x[1], x[3]);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) P2::mma(sc[g][nt], x, qf[nt][c + w][0], qf[nt][c + w][1]);
+            }
           }
         }
+      const float none = __int_as_float(0xff800000);
+      const bool full = key >= cur.s.first && key + 16 * M <= cur.s.len;
+#pragma unroll
+      for (int g = 0; g < M; ++g)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[g][nt][e] *= q_scale[nt][e & 1];
+      if (!full) {
+#pragma unroll
+        for (int g = 0; g < M; ++g) {
+          const int t0 = key + 16 * g + row4, t1 = t0 + 8;
+          const bool ok0 = t0 >= cur.s.first && t0 < cur.s.len, ok1 = t1 >= cur.s.first && t1 < cur.s.len;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (!(e < 2 ? ok0 : ok1)) sc[g][nt][e] = none;
+        }
       }
-      const int t0 = key + row4, t1 = t0 + 8;
-      const bool full = key >= cur.s.first && key + 16 <= cur.s.len;
+      float top[NT][2];  // largest of this lane's scores, per head
       bool up = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[nt][e] *= q_scale[nt][e & 1];
-      if (!full) {
-        const bool ok0 = t0 >= cur.s.first && t0 < cur.s.len, ok1 = t1 >= cur.s.first && t1 < cur.s.len;
+        for (int e = 0; e < 2; ++e) {
+          top[nt][e] = fmaxf(sc[0][nt][e], sc[0][nt][e + 2]);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (!(e < 2 ? ok0 : ok1)) sc[nt][e] = __int_as_float(0xff800000);
-      }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-        up = up || fmaxf(sc[nt][0], sc[nt][2]) > m[nt][0] || fmaxf(sc[nt][1], sc[nt][3]) > m[nt][1];
+          for (int g = 1; g < M; ++g) top[nt][e] = fmaxf(top[nt][e], fmaxf(sc[g][nt][e], sc[g][nt][e + 2]));
+          up = up || top[nt][e] > m[nt][e];
+        }
       if (p.scores != nullptr) {
         const int g0 = cur.block * S::HEADS, live_heads = min(S::HEADS, p.group - g0);
         float* out = p.scores +
                      ((static_cast<long long>(cur.b) * p.cache.kv_heads + cur.h) * p.capacity) * p.group + g0;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int g = 0; g < M; ++g)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int n = nt * 8 + col4 * 2 + (e & 1);
-            const int t = e < 2 ? t0 : t1;
-            if (n < live_heads && t >= cur.s.first && t < cur.s.len)
-              out[static_cast<long long>(t) * p.group + n] = sc[nt][e];
-          }
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int n = nt * 8 + col4 * 2 + (e & 1);
+              const int t = key + 16 * g + row4 + (e < 2 ? 0 : 8);
+              if (n < live_heads && t >= cur.s.first && t < cur.s.len)
+                out[static_cast<long long>(t) * p.group + n] = sc[g][nt][e];
+            }
       }
       if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float v = fmaxf(m[nt][e], fmaxf(sc[nt][e], sc[nt][e + 2]));
+            float v = fmaxf(m[nt][e], top[nt][e]);
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, x));
             // All scores -inf so far: nothing to rescale.
@@ -587,55 +639,57 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
       }
       // P^T as the B operand: transposed 8 x 8 blocks of the score fragments; two 16-bit
       // halves whose sum is p to fp32's precision (fp16: to 2^-25 of the largest weight).
-      uint32_t ph[NT][2], pl[NT][2];
+      uint32_t ph[M][NT][2], pl[M][NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
+        const float mm0 = m[nt][0] == none ? 0.f : m[nt][0];
+        const float mm1 = m[nt][1] == none ? 0.f : m[nt][1];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float mm0 = m[nt][0] == __int_as_float(0xff800000) ? 0.f : m[nt][0];
-          const float mm1 = m[nt][1] == __int_as_float(0xff800000) ? 0.f : m[nt][1];
-          const float p0 = dev::ex2_approx(sc[nt][2 * e] - mm0);
-          const float p1 = dev::ex2_approx(sc[nt][2 * e + 1] - mm1);
-          l[nt][0] += p0;
-          l[nt][1] += p1;
-          const uint32_t hi = P2::pack(p0, p1);
-          const float2 f = P2::unpack(hi);
-          ph[nt][e] = transpose_8x8(hi);
-          pl[nt][e] = transpose_8x8(P2::pack(p0 - f.x, p1 - f.y));
-        }
+        for (int g = 0; g < M; ++g)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float p0 = dev::ex2_approx(sc[g][nt][2 * e] - mm0);
+            const float p1 = dev::ex2_approx(sc[g][nt][2 * e + 1] - mm1);
+            l[nt][0] += p0;
+            l[nt][1] += p1;
+            const uint32_t hi = P2::pack(p0, p1);
+            const float2 f = P2::unpack(hi);
+            ph[g][nt][e] = transpose_8x8(hi);
+            pl[g][nt][e] = transpose_8x8(P2::pack(p0 - f.x, p1 - f.y));
+          }
       }
       // O^T += V^T P^T: rows = head elements. 16-bit: tile kk holds elements 16 kk + row.
       // e4m3: ldmatrix moves pairs of elements; tile row j < 8 is element 16 kk + 2 j, row
       // 8 + j element 16 kk + 2 j + 1.
-      if (!F8) {
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-          uint32_t a[4];
-          ldsm_x4_t(a, (vs + v_lane) ^ (kk << 5));
+      for (int g = 0; g < M; ++g) {
+        const uint32_t vg = vs + v_lane;
+        if constexpr (!F8) {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            P2::mma(o[nt][kk], a, ph[nt][0], ph[nt][1]);
-            P2::mma(o[nt][kk], a, pl[nt][0], pl[nt][1]);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int k2 = 0; k2 < KK; k2 += 2) {
-          uint32_t a[4];
-          ldsm_x4_t(a, (vs + v_lane) ^ (k2 << 4));
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            const uint32_t lo = __byte_perm(a[2 * w], 0u, 0x3120);
-            const uint32_t hi = __byte_perm(a[2 * w + 1], 0u, 0x3120);
-            uint32_t x[4];
-            x[0] = e4m3_to_half2(static_cast<uint16_t>(lo));
-            x[1] = e4m3_to_half2(static_cast<uint16_t>(lo >> 16));
-            x[2] = e4m3_to_half2(static_cast<uint16_t>(hi));
-            x[3] = e4m3_to_half2(static_cast<uint16_t>(hi >> 16));
+          for (int kk = 0; kk < KK; ++kk) {
+            uint32_t a[4];
+            ldsm_x4_t(a, (vg ^ (kk << 5)) + g * 16 * ROWB);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              P2::mma(o[nt][k2 + w], x, ph[nt][0], ph[nt][1]);
-              P2::mma(o[nt][k2 + w], x, pl[nt][0], pl[nt][1]);
+              P2::mma(o[nt][kk], a, ph[g][nt][0], ph[g][nt][1]);
+              P2::mma(o[nt][kk], a, pl[g][nt][0], pl[g][nt][1]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int k2 = 0; k2 < KK; k2 += 2) {
+            uint32_t a[4];
+            ldsm_x4_t(a, (vg ^ (k2 << 4)) + g * 16 * ROWB);
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              uint32_t x[4];
+              e4m3_to_half(__byte_perm(a[2 * w], 0u, 0x3120), x[0], x[1]);
+              e4m3_to_half(__byte_perm(a[2 * w + 1], 0u, 0x3120), x[2], x[3]);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                P2::mma(o[nt][k2 + w], x, ph[g][nt][0], ph[g][nt][1]);
+                P2::mma(o[nt][k2 + w], x, pl[g][nt][0], pl[g][nt][1]);
+              }
             }
           }
         }
@@ -657,7 +711,7 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
     const int head0 = done.h * p.group + done.block * S::HEADS;
     const int slot = 2 * cta + (seg_begin == 0 ? 1 : 0);
     if (i + 1 < n_tiles) {
-      paged_next_item(p, cur);
+      paged_next_item<S::TILE>(p, cur);
       load_q(cur);
       seg_begin = 0;
     }

@@ -61,10 +61,12 @@ struct Quad<fp8_e4m3> {
   }
 };
 
-// A sequence's keys: [first, len), cut into tiles from `base` (first rounded down to 16).
+// A sequence's keys: [first, len), cut into tiles of TILE from `base` (first rounded down to
+// 16).
 struct PagedSpan {
   int len, first, base, tiles;
 };
+template <int TILE>
 __device__ __forceinline__ PagedSpan paged_span(const PagedAttnParams& p, int b) {
   PagedSpan s;
   int n = p.seq_lens[b];
@@ -72,7 +74,7 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedAttnParams& p, int b)
   s.len = n;
   s.first = p.window > 0 && n > p.window ? n - p.window : 0;
   s.base = s.first & ~15;
-  s.tiles = n > 0 ? (n - s.base + kPagedTile - 1) / kPagedTile : 0;
+  s.tiles = n > 0 ? (n - s.base + TILE - 1) / TILE : 0;
   return s;
 }
 

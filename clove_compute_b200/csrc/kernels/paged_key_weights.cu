@@ -18,7 +18,7 @@ __global__ void __launch_bounds__(256) paged_key_weights_kernel(const PagedAttnP
   for (long long bh = blockIdx.y; bh < rows; bh += gridDim.y) {
     const int b = static_cast<int>(bh / p.cache.kv_heads);
     const int h = static_cast<int>(bh - static_cast<long long>(b) * p.cache.kv_heads);
-    const PagedSpan s = paged_span(p, b);
+    const PagedSpan s = paged_span<kPagedTile>(p, b);
     const float* lse2 = p.lse2 + static_cast<long long>(b) * p.heads + h * p.group;
     for (int t = s.first + static_cast<int>(blockIdx.x * blockDim.x + threadIdx.x); t < s.len;
          t += static_cast<int>(gridDim.x * blockDim.x)) {

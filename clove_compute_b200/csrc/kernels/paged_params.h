@@ -46,7 +46,7 @@ struct RopeParams {
 };
 
 // paged_attention_sm100.cuh
-constexpr int kPagedTile = 64;  // keys per CTA step
+constexpr int kPagedTile = 64;  // keys per CTA step, at least
 constexpr int kPagedCounters = 1 << 18;
 struct PagedAttnParams {
   const void* q;
