@@ -18,7 +18,6 @@ import torch
 from ._lib import PagedCacheStruct, check, fastcall
 
 DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float8_e4m3fn: 2}
-_16BIT = (torch.float16, torch.bfloat16)
 
 
 class PagedCache:
@@ -51,7 +50,8 @@ class PagedCache:
         self.K, self.V, self.layout = K, V, layout
         self.num_pages, self.page_size = K.shape[0], K.shape[tok]
         self.num_kv_heads, self.head_dim = K.shape[head], K.shape[3]
-        self.dtype, self.device = K.dtype, K.device
+        self.dtype, self.device, self.index = K.dtype, K.device, K.get_device()
+        self.weights_shape = (self.num_pages, self.num_kv_heads, self.page_size)  # of key_weights
         self.k_scale, self.v_scale = float(k_scale), float(v_scale)
         self.struct = PagedCacheStruct(K.data_ptr(), V.data_ptr(), self.num_pages, self.page_size,
                                        self.num_kv_heads, self.head_dim, K.stride(0), K.stride(tok),
@@ -59,82 +59,70 @@ class PagedCache:
         self._address = ctypes.addressof(self.struct)
 
 
-def _ints(t, name, device, shape):
-    if t.dtype != torch.int32:
-        raise TypeError(f"{name} must be torch.int32, got {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} must be on {device}")
-    if t.shape != shape:
-        raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
-    return t.data_ptr()
+# Checks of the operands. They run on every call of a decode step, so each attribute is
+# read once and devices are compared by index.
+def _no(t, name, want):
+    raise ValueError(f"{name} must be {want}, got {tuple(t.shape)} on {t.device}")
 
 
-def _table(t, name, device, batch):
-    if t.dtype != torch.int32:
-        raise TypeError(f"{name} must be torch.int32, got {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} must be on {device}")
-    if t.dim() != 2 or t.shape[0] != batch:
-        raise ValueError(f"{name} must be [{batch}, pages], got {tuple(t.shape)}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
-        raise ValueError(f"{name}'s rows must be contiguous")
-    return t.data_ptr()
-
-
-def _heads(t, name, dtype, device, shape):
-    """A [rows, heads, D] operand whose rows are contiguous; its row stride."""
-    if t.dtype != dtype:
+def _dense(t, name, dtype, index, shape):
+    """A contiguous tensor of this type and shape on GPU `index`; its address."""
+    if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} must be on {device}")
-    if t.shape != shape:
-        raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
+    if t.get_device() != index or t.shape != shape or not t.is_contiguous():
+        _no(t, name, f"contiguous {tuple(shape)} on GPU {index}")
+    return t.data_ptr()
+
+
+def _table(t, name, index, batch):
+    """A [batch, pages] int32 tensor with contiguous rows; its address, pages and row stride."""
+    if t.dtype is not torch.int32:
+        raise TypeError(f"{name} must be torch.int32, got {t.dtype}")
     s = t.stride()
-    if s[2] != 1 or (shape[1] > 1 and s[1] != shape[2]):
-        raise ValueError(f"{name}: the last two dimensions must be contiguous")
+    if t.get_device() != index or len(s) != 2 or t.shape[0] != batch or (s[1] != 1 and t.shape[1] > 1):
+        _no(t, name, f"[{batch}, pages] with contiguous rows on GPU {index}")
+    return t.data_ptr(), t.shape[1], s[0]
+
+
+def _heads(t, name, dtype, index, shape):
+    """A [rows, heads, D] operand whose rows are contiguous; its row stride."""
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    s = t.stride()
+    if t.get_device() != index or t.shape != shape or s[2] != 1 or (s[1] != shape[2] and shape[1] > 1):
+        _no(t, name, f"{tuple(shape)} with contiguous rows on GPU {index}")
     return s[0] if shape[0] > 1 else shape[1] * shape[2]
 
 
-def _floats(t, name, device, shape):
-    if t.dtype != torch.float32:
-        raise TypeError(f"{name} must be torch.float32, got {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} must be on {device}")
-    if t.shape != shape:
-        raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
-    return t.data_ptr()
-
-
 def _operand(t, name):
-    if not isinstance(t, torch.Tensor) or t.dtype not in _16BIT:
+    """(dtype code, GPU index, shape) of the call's first operand."""
+    code = DTYPES.get(t.dtype, 2) if isinstance(t, torch.Tensor) else 2
+    if code == 2:
         raise TypeError(f"{name} must be an fp16 or bf16 tensor")
-    if not t.is_cuda:
+    index, shape = t.get_device(), t.shape
+    if index < 0:
         raise ValueError(f"{name} must be a CUDA tensor")
-    if t.dim() != 3:
-        raise ValueError(f"{name} must be 3-D, got shape {tuple(t.shape)}")
+    if len(shape) != 3:
+        raise ValueError(f"{name} must be 3-D, got shape {tuple(shape)}")
+    return code, index, shape
 
 
-# The current stream's handle, without the Stream object that torch.cuda.current_stream()
-# builds (2 us a call).
-_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+# The current stream's handle and device without the objects that torch.cuda's own
+# functions build or look up (3 us a call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def _on(fn, device, stream, *args):
-    """fn(stream handle, *args) with `device` current; an explicit stream is current while
-    outputs are allocated, so that their memory belongs to it."""
-    if stream is not None:
-        s = stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(int(stream), device=device)
-        with torch.cuda.device(device), torch.cuda.stream(s):
+def _elsewhere(fn, index, stream, *args):
+    """fn(stream handle, ...) for a stream or device other than the current one. The stream
+    is current while outputs are allocated, so that their memory belongs to it."""
+    with torch.cuda.device(index):
+        if stream is None:
+            return fn(_raw_stream(index), *args)
+        s = stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(int(stream), device=index)
+        with torch.cuda.stream(s):
             return fn(s.cuda_stream, *args)
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return fn(_current_stream(device.index), *args)
-    return fn(_current_stream(device.index), *args)
 
 
 def rope_table(length: int, rotary_dim: int, theta: float = 10000.0, device="cuda") -> torch.Tensor:
@@ -158,55 +146,58 @@ def qk_norm_rope(Q, K, rope_table, positions, q_weight=None, k_weight=None, eps:
     (Q_out, K_out); with a cache K_out is None unless it was given. Q_out may be Q and
     K_out K. Negative positions mark padding tokens (nothing written), negative slots
     tokens that are not stored; other slots must differ."""
-    _operand(Q, "Q")
-    _operand(K, "K")
-    return _on(_qk_norm_rope, Q.device, stream, Q, K, rope_table, positions, q_weight, k_weight, eps,
-               interleaved, V, cache, slots, Q_out, K_out)
+    code, index, shape = _operand(Q, "Q")
+    args = (code, index, shape, Q, K, rope_table, positions, q_weight, k_weight, eps, interleaved, V, cache,
+            slots, Q_out, K_out)
+    if stream is not None or index != _current_device():
+        return _elsewhere(_qk_norm_rope, index, stream, *args)
+    return _qk_norm_rope(_raw_stream(index), *args)
 
 
-def _qk_norm_rope(stream, Q, K, table, positions, q_weight, k_weight, eps, interleaved, V, cache, slots,
-                  Q_out, K_out):
-    dtype, device = Q.dtype, Q.device
-    T, H, D = Q.shape
-    Hkv = K.shape[1]
-    kv = (T, Hkv, D)
-    qs = _heads(Q, "Q", dtype, device, (T, H, D))
-    ks = _heads(K, "K", dtype, device, kv)
-    if table.dim() != 2:
+def _qk_norm_rope(stream, code, index, shape, Q, K, table, positions, q_weight, k_weight, eps, interleaved, V,
+                  cache, slots, Q_out, K_out):
+    dtype = Q.dtype
+    T, H, D = shape
+    kv = K.shape
+    if len(kv) != 3 or kv[0] != T or kv[2] != D:
+        raise ValueError(f"K must be [{T}, kv_heads, {D}], got {tuple(kv)}")
+    qs = _heads(Q, "Q", dtype, index, shape)
+    ks = _heads(K, "K", dtype, index, kv)
+    ts = table.shape
+    if len(ts) != 2:
         raise ValueError("rope_table must be [positions, rotary_dim]")
-    tp = _floats(table, "rope_table", device, table.shape)
-    pp = _ints(positions, "positions", device, (T,))
+    tp = _dense(table, "rope_table", torch.float32, index, ts)
+    pp = _dense(positions, "positions", torch.int32, index, (T,))
     wq = wk = None
-    if (q_weight is None) != (k_weight is None):
+    if q_weight is not None and k_weight is not None:
+        wq = _dense(q_weight, "q_weight", dtype, index, (D,))
+        wk = _dense(k_weight, "k_weight", dtype, index, (D,))
+    elif q_weight is not k_weight:
         raise ValueError("q_weight and k_weight: both or neither")
-    if q_weight is not None:
-        for w, n in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-            if w.dtype != dtype or w.device != device or w.shape != (D,) or not w.is_contiguous():
-                raise ValueError(f"{n} must be a contiguous [{D}] tensor of {dtype} on {device}")
-        wq, wk = q_weight.data_ptr(), k_weight.data_ptr()
-    vs = 0
-    vp = sp = ref = None
+    vs = kos = 0
+    vp = sp = ref = kp = None
     if cache is not None:
         if V is None or slots is None:
             raise ValueError("a cache needs V and slots")
-        if cache.device != device:
-            raise ValueError(f"the cache must be on {device}")
-        vs = _heads(V, "V", dtype, device, kv)
-        vp, sp, ref = V.data_ptr(), _ints(slots, "slots", device, (T,)), cache._address
+        if cache.index != index:
+            raise ValueError(f"the cache must be on GPU {index}")
+        vs = _heads(V, "V", dtype, index, kv)
+        vp, sp, ref = V.data_ptr(), _dense(slots, "slots", torch.int32, index, (T,)), cache._address
     elif V is not None or slots is not None:
         raise ValueError("V and slots need a cache")
+    elif K_out is None:
+        K_out = torch.empty_like(K, memory_format=torch.contiguous_format)
     if Q_out is None:
-        Q_out = torch.empty((T, H, D), dtype=dtype, device=device)
+        Q_out = torch.empty_like(Q, memory_format=torch.contiguous_format)
         qos = H * D
     else:
-        qos = _heads(Q_out, "Q_out", dtype, device, (T, H, D))
-    if K_out is None and cache is None:
-        K_out = torch.empty(kv, dtype=dtype, device=device)
-    kos = _heads(K_out, "K_out", dtype, device, kv) if K_out is not None else 0
+        qos = _heads(Q_out, "Q_out", dtype, index, shape)
+    if K_out is not None:
+        kos = _heads(K_out, "K_out", dtype, index, kv)
+        kp = K_out.data_ptr()
     rc = fastcall().qk_norm_rope(
-        Q.data_ptr(), K.data_ptr(), vp, qs, ks, vs, wq, wk, eps, tp, table.shape[0], table.shape[1],
-        1 if interleaved else 0, pp, ref, sp, Q_out.data_ptr(), qos,
-        K_out.data_ptr() if K_out is not None else None, kos, T, H, Hkv, D, DTYPES[dtype], stream)
+        Q.data_ptr(), K.data_ptr(), vp, qs, ks, vs, wq, wk, eps, tp, ts[0], ts[1], 1 if interleaved else 0,
+        pp, ref, sp, Q_out.data_ptr(), qos, kp, kos, T, H, kv[1], D, code, stream)
     if rc:
         check(rc)
     return Q_out, K_out
@@ -223,37 +214,38 @@ def paged_attention(Q, cache: PagedCache, page_table, seq_lens, scale: float | N
     [pages, kv_heads, page_size] fp32, if given, gets the softmax weight of every attended
     key, summed over its query heads (added with accumulate=True); no page may then be in
     two sequences. scale defaults to 1/sqrt(D). An empty sequence gives zeros and -inf."""
-    _operand(Q, "Q")
-    return _on(_paged_attention, Q.device, stream, Q, cache, page_table, seq_lens, scale, window, lse,
-               key_weights, accumulate, O)
+    code, index, shape = _operand(Q, "Q")
+    args = (code, index, shape, Q, cache, page_table, seq_lens, scale, window, lse, key_weights, accumulate, O)
+    if stream is not None or index != _current_device():
+        return _elsewhere(_paged_attention, index, stream, *args)
+    return _paged_attention(_raw_stream(index), *args)
 
 
-def _paged_attention(stream, Q, cache, page_table, seq_lens, scale, window, lse, key_weights, accumulate, O):
-    dtype, device = Q.dtype, Q.device
-    B, H, D = Q.shape
-    if cache.device != device:
-        raise ValueError(f"the cache must be on {device}")
+def _paged_attention(stream, code, index, shape, Q, cache, page_table, seq_lens, scale, window, lse,
+                     key_weights, accumulate, O):
+    dtype = Q.dtype
+    B, H, D = shape
+    if cache.index != index:
+        raise ValueError(f"the cache must be on GPU {index}")
     if D != cache.head_dim:
         raise ValueError(f"Q has head_dim {D}, the cache {cache.head_dim}")
-    qs = _heads(Q, "Q", dtype, device, (B, H, D))
-    pt = _table(page_table, "page_table", device, B)
-    sl = _ints(seq_lens, "seq_lens", device, (B,))
-    if O is None:
-        O = torch.empty((B, H, D), dtype=dtype, device=device)
-        os = H * D
-    else:
-        os = _heads(O, "O", dtype, device, (B, H, D))
-    lp = _floats(lse, "lse", device, (B, H)) if lse is not None else None
+    qs = _heads(Q, "Q", dtype, index, shape)
+    pt, pages, ps = _table(page_table, "page_table", index, B)
+    sl = _dense(seq_lens, "seq_lens", torch.int32, index, (B,))
+    lp = _dense(lse, "lse", torch.float32, index, (B, H)) if lse is not None else None
     kw = None
     if key_weights is not None:
-        kw = _floats(key_weights, "key_weights", device,
-                     (cache.num_pages, cache.num_kv_heads, cache.page_size))
+        kw = _dense(key_weights, "key_weights", torch.float32, index, cache.weights_shape)
     elif accumulate:
         raise ValueError("accumulate needs key_weights")
+    if O is None:
+        O = torch.empty_like(Q, memory_format=torch.contiguous_format)
+        os = H * D
+    else:
+        os = _heads(O, "O", dtype, index, shape)
     rc = fastcall().paged_attention(
-        Q.data_ptr(), qs, cache._address, pt, page_table.stride(0), page_table.shape[1], sl, O.data_ptr(), os,
-        lp, kw, 1 if accumulate else 0, B, H, D ** -0.5 if scale is None else scale, window,
-        DTYPES[dtype], stream)
+        Q.data_ptr(), qs, cache._address, pt, ps, pages, sl, O.data_ptr(), os, lp, kw, 1 if accumulate else 0,
+        B, H, D ** -0.5 if scale is None else scale, window, code, stream)
     if rc:
         check(rc)
     return O
@@ -266,27 +258,26 @@ def evict_cache(cache: PagedCache, key_weights, page_table, seq_lens, dst_table,
     index). Their K, V and weights are copied, in order, to the fresh pages of dst_table
     [B, >= ceil(budget / page_size)], none of which may still be in use. Returns (kept
     [B, kv_heads, budget] int32 -- indices, -1 behind them -- and the new lengths [B])."""
-    if not cache.K.is_cuda:
-        raise ValueError("the cache must be on a CUDA device")
-    return _on(_evict_cache, cache.device, stream, cache, key_weights, page_table, seq_lens, dst_table,
-               budget, recent)
+    index = cache.index
+    args = (index, cache, key_weights, page_table, seq_lens, dst_table, budget, recent)
+    if stream is not None or index != _current_device():
+        return _elsewhere(_evict_cache, index, stream, *args)
+    return _evict_cache(_raw_stream(index), *args)
 
 
-def _evict_cache(stream, cache, key_weights, page_table, seq_lens, dst_table, budget, recent):
-    device = cache.device
+def _evict_cache(stream, index, cache, key_weights, page_table, seq_lens, dst_table, budget, recent):
     B = seq_lens.shape[0]
-    kw = _floats(key_weights, "key_weights", device,
-                 (cache.num_pages, cache.num_kv_heads, cache.page_size))
-    pt = _table(page_table, "page_table", device, B)
-    dt = _table(dst_table, "dst_table", device, B)
-    sl = _ints(seq_lens, "seq_lens", device, (B,))
+    kw = _dense(key_weights, "key_weights", torch.float32, index, cache.weights_shape)
+    pt, pages, ps = _table(page_table, "page_table", index, B)
+    dt, dst_pages, ds = _table(dst_table, "dst_table", index, B)
+    sl = _dense(seq_lens, "seq_lens", torch.int32, index, (B,))
     if budget <= 0:
         raise ValueError("budget must be positive")
-    kept = torch.empty((B, cache.num_kv_heads, budget), dtype=torch.int32, device=device)
-    new_lens = torch.empty((B,), dtype=torch.int32, device=device)
+    kept = seq_lens.new_empty((B, cache.num_kv_heads, budget))
+    new_lens = torch.empty_like(seq_lens)
     rc = fastcall().evict_cache(
-        cache._address, kw, pt, page_table.stride(0), page_table.shape[1], sl, dt, dst_table.stride(0),
-        dst_table.shape[1], kept.data_ptr(), new_lens.data_ptr(), B, budget, recent, stream)
+        cache._address, kw, pt, ps, pages, sl, dt, ds, dst_pages, kept.data_ptr(), new_lens.data_ptr(), B,
+        budget, recent, stream)
     if rc:
         check(rc)
     return kept, new_lens
