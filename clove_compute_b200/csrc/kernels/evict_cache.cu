@@ -55,14 +55,14 @@ template <bool LONG>
 __global__ void __launch_bounds__(kEvictThreads, 1) evict_select_kernel(const EvictParams p, int cs) {
   extern __shared__ uint32_t cached[];
   __shared__ __align__(16) uint32_t hist[2][kEvictBins];
+  __shared__ uint32_t coarse[2][kEvictWarps];
   __shared__ uint32_t counts[2];  // this CTA's keys above the threshold, and equal to it
   __shared__ uint32_t warp_a[kEvictWarps], warp_b[kEvictWarps];
   __shared__ uint32_t pick[2];  // chosen digit, keys of larger digits
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = blockIdx.x % cs;
-  const long long row = blockIdx.x / cs;
-  const int b = static_cast<int>(row / p.cache.kv_heads);
-  const int h = static_cast<int>(row - static_cast<long long>(b) * p.cache.kv_heads);
+  const int row = static_cast<int>(blockIdx.x) / cs;
+  const int b = row / p.cache.kv_heads, h = row - b * p.cache.kv_heads;
   const int page_mask = (1 << p.cache.page_shift) - 1;
   dev::grid_dependency_wait();
   dev::allow_dependent_launch();
@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(kEvictThreads, 1) evict_select_kernel(const Ev
     if (tid == 0) dev::record_error(dev::kDevErrBadIndex);
     n = n < 0 ? 0 : p.capacity;
   }
-  int* kept = p.kept + row * p.budget;
+  int* kept = p.kept + static_cast<long long>(row) * p.budget;
   if (h == 0 && rank == 0 && tid == 0) p.new_lens[b] = min(n, p.budget);
   if (n <= p.budget) {
     for (int j = static_cast<int>(rank) * kEvictThreads + tid; j < p.budget; j += cs * kEvictThreads)
@@ -82,10 +82,11 @@ __global__ void __launch_bounds__(kEvictThreads, 1) evict_select_kernel(const Ev
   const int m = n - p.recent, want = p.budget - p.recent;
   const int per = (m + cs - 1) / cs;
   const int s0 = min(m, static_cast<int>(rank) * per), sn = min(m, s0 + per) - s0;
-  // Weights of keys of the slice, looked up for sixteen keys at a time before any of them is
+  // Weights of keys of the slice, looked up for four keys at a time before any of them is
   // read: first all pages (into the keys' places), then all weights. The loads are
   // unconditional (index and page clamped, the result dropped), so that none waits for
-  // another; a bad page counts as weight 0.
+  // another; a bad page counts as weight 0. (Sixteen at a time take 3 us more on 4096 keys,
+  // fetching the instructions, and 0.6 us less on 131071.)
   bool bad = false;
   auto page_at = [&](int i) { return p.page_table[b * p.table_stride + ((s0 + i) >> p.cache.page_shift)]; };
   auto good = [&](int pg) { return pg >= 0 && pg < p.cache.num_pages; };
@@ -96,7 +97,7 @@ __global__ void __launch_bounds__(kEvictThreads, 1) evict_select_kernel(const Ev
   };
   for (int i = tid; i < kEvictBins; i += kEvictThreads) hist[0][i] = 0;
   const int in_smem = LONG ? min(sn, kEvictCached) : sn;
-  constexpr int DEEP = 16;
+  constexpr int DEEP = 4;
   for (int i0 = tid; i0 < in_smem; i0 += DEEP * kEvictThreads) {
     int pg[DEEP];
 #pragma unroll
@@ -153,50 +154,55 @@ __global__ void __launch_bounds__(kEvictThreads, 1) evict_select_kernel(const Ev
       if (lane == lead) atomicAdd(&mine[d0], static_cast<uint32_t>(__popc(same)));
       else if (in && digit != d0) atomicAdd(&mine[digit], 1u);
     }
-    // All CTAs' histograms of this digit are complete, and those of the digit before have
-    // been read.
-    dev::cluster_sync_all();
-    // Thread t holds the digits 2047 - 2 t and 2046 - 2 t: from the largest down (digits
-    // above the mask are empty).
-    constexpr int PER = kEvictBins / kEvictThreads;
-    static_assert(PER == 2, "one 8-byte load per thread and CTA");
-    const int low = kEvictBins - PER * (tid + 1);
-    uint32_t c[PER] = {0, 0};
-    if (static_cast<uint32_t>(low) <= mask) {
-      uint2 x[8];
-#pragma unroll
-      for (int r = 0; r < 8; ++r)
-        x[r] = r < cs ? ld_cluster_v2(&mine[low], static_cast<uint32_t>(r)) : make_uint2(0u, 0u);
-#pragma unroll
-      for (int r = 0; r < 8; ++r) c[0] += x[r].y, c[1] += x[r].x;
-    }
-    const uint32_t own = c[0] + c[1];
-    hist[(d & 1) ^ 1][low] = hist[(d & 1) ^ 1][low + 1] = 0;
-    uint32_t inc = own;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += v;
-    }
-    if (lane == 31) warp_a[warp] = inc;
-    if (tid == 0) pick[0] = mask, pick[1] = 0u;  // left == 0: nothing is wanted
     __syncthreads();
-    uint32_t run = inc - own;
-    {  // the warps before this one: one lane each
-      uint32_t v = lane < warp ? warp_a[lane] : 0u;
+    // Sums of 64 bins each, one per warp, from the largest down.
+    {
+      const int bin = kEvictBins - 64 * (warp + 1) + 2 * lane;
+      uint32_t v = mine[bin] + mine[bin + 1];
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      run += v;
+      if (lane == 0) coarse[d & 1][warp] = v;
+      hist[(d & 1) ^ 1][bin] = hist[(d & 1) ^ 1][bin + 1] = 0;  // for the next digit
     }
-    // The `left`-th largest key lies in one thread's digits.
-    if (run < left && run + own >= left) {
+    // All CTAs' histograms of this digit are complete, and those of the digit before have
+    // been read. (The other histogram was read before the last barrier: it may be cleared.)
+    dev::cluster_sync_all();
+    if (warp == 0) {
+      // Warp 0 finds the `left`-th largest key's 64 bins, then its bin, adding up the CTAs'
+      // counts of those alone.
+      auto scan_from_top = [&](uint32_t own) {
+        uint32_t inc = own;
 #pragma unroll
-      for (int e = 0; e < PER; ++e) {
-        if (run < left && run + c[e] >= left) {
-          pick[0] = static_cast<uint32_t>(kEvictBins - 1 - PER * tid - e);
-          pick[1] = run;
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
+          if (lane >= o) inc += v;
         }
-        run += c[e];
+        return inc - own;
+      };
+      uint32_t x[8], own = 0;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) x[r] = r < cs ? ld_cluster_u32(&coarse[d & 1][lane], static_cast<uint32_t>(r)) : 0u;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) own += x[r];
+      uint32_t run = scan_from_top(own);
+      unsigned hit = __ballot_sync(0xffffffffu, run < left && run + own >= left);
+      const int block = hit ? __ffs(hit) - 1 : 0;  // (left == 0: nothing is wanted, digit `mask`)
+      run = __shfl_sync(0xffffffffu, run, block);
+      const int low = kEvictBins - 64 * block - 2 * (lane + 1);
+      uint2 y[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        y[r] = r < cs ? ld_cluster_v2(&mine[low], static_cast<uint32_t>(r)) : make_uint2(0u, 0u);
+      uint32_t c0 = 0, c1 = 0;  // the larger and the smaller of the lane's two bins
+#pragma unroll
+      for (int r = 0; r < 8; ++r) c0 += y[r].y, c1 += y[r].x;
+      run += scan_from_top(c0 + c1);
+      if (left == 0) {
+        if (lane == 0) pick[0] = mask, pick[1] = 0u;
+      } else if (run < left && run + c0 + c1 >= left) {
+        const bool first = run + c0 >= left;
+        pick[0] = static_cast<uint32_t>(first ? low + 1 : low);
+        pick[1] = first ? run : run + c0;
       }
     }
     __syncthreads();
@@ -382,10 +388,10 @@ int launch_evict_cache(const kern::EvictParams& p, const DeviceInfo& dev, cudaSt
     g_evict_attr.fetch_or(bit, std::memory_order_acq_rel);
   }
   // CTAs per (sequence, head): up to 8 while all of them fit on the GPU at once (one per
-  // SM) and each still has a strip of 1024 keys.
+  // SM) and each has 4096 keys, four per thread.
   const long long rows = static_cast<long long>(p.batch) * p.cache.kv_heads;
   int cs = 1;
-  while (cs < 8 && rows * cs * 2 <= dev.num_sms && p.capacity > cs * kern::kEvictThreads) cs *= 2;
+  while (cs < 8 && rows * cs * 2 <= dev.num_sms && p.capacity > cs * 4 * kern::kEvictThreads) cs *= 2;
   if (rows * cs > 0x7fffffffLL) return fail(CLOVE_ERR_UNSUPPORTED, "evict_cache: batch x heads exceeds 2^31");
   const int slice = (p.capacity + cs - 1) / cs;
   cudaLaunchAttribute la[2];

@@ -449,7 +449,7 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
   };
   if (whole_pages) win = window(ld, ld.tile);
   enter();
-#pragma unroll
+#pragma unroll 1  // (instructions fetched once)
   for (int i = 0; i < S::STAGES - 1; ++i) issue(i);
 
   // ldmatrix addresses within a chunk; piece c is reached by an exclusive or with c << 4.
