@@ -239,57 +239,45 @@ __device__ __forceinline__ void paged_store(const PagedAttnParams& p, int b, int
 }
 
 // Adds up the partial results of CTAs c0 .. c1 (c0's second, the others' first) with a
-// running maximum, eight parts of two results at a time in flight, and stores the item.
+// running maximum, kPagedJoin parts in flight, and stores the item. (Short code on purpose:
+// it runs once or twice per CTA, and fetching its instructions is much of its time.)
+constexpr int kPagedJoin = 8;
 template <typename T, int D, int HEADS>
 __device__ __forceinline__ void paged_join(const PagedAttnParams& p, int c0, int c1, int live_heads, int b,
                                            int head0) {
-  constexpr int THREADS = kPagedWarps * 32, BATCH = 8;
   const int work = live_heads * (D / 4);  // four elements of a head each
-  for (int i0 = static_cast<int>(threadIdx.x); i0 < work; i0 += 2 * THREADS) {
-    float top[2], sum[2] = {0.f, 0.f}, v[2][4] = {};
-    top[0] = top[1] = __int_as_float(0xff800000);
-    for (int c = c0; c <= c1; c += BATCH) {
-      float m[2][BATCH], l[2][BATCH];
-      float4 x[2][BATCH];
+#pragma unroll 1
+  for (int idx = static_cast<int>(threadIdx.x); idx < work; idx += kPagedWarps * 32) {
+    const int n = idx / (D / 4), d = (idx - n * (D / 4)) * 4;
+    float top = __int_as_float(0xff800000), sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int c = c0; c <= c1; c += kPagedJoin) {
+      float m[kPagedJoin], l[kPagedJoin];
+      float4 x[kPagedJoin];
 #pragma unroll
-      for (int w = 0; w < 2; ++w)
+      for (int k = 0; k < kPagedJoin; ++k) {
+        // (Past the last part: the last one again, emptied.)
+        const int ck = min(c + k, c1), at = (2 * ck + (ck == c0 ? 1 : 0)) * HEADS + n;
+        m[k] = __ldcg(p.part_m + at);
+        l[k] = __ldcg(p.part_l + at);
+        x[k] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * D + d));
+        if (c + k > c1) l[k] = 0.f, x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      float t = top;
 #pragma unroll
-        for (int k = 0; k < BATCH; ++k) {
-          const int idx = i0 + w * THREADS, n = idx / (D / 4), d = (idx - n * (D / 4)) * 4;
-          m[w][k] = __int_as_float(0xff800000);
-          l[w][k] = 0.f;
-          x[w][k] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (idx < work && c + k <= c1) {
-            const int at = (2 * (c + k) + (c + k == c0 ? 1 : 0)) * HEADS + n;
-            m[w][k] = __ldcg(p.part_m + at);
-            l[w][k] = __ldcg(p.part_l + at);
-            x[w][k] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * D + d));
-          }
-        }
+      for (int k = 0; k < kPagedJoin; ++k) t = fmaxf(t, m[k]);
+      const float f0 = top == t ? 1.f : dev::ex2_approx(top - t);
+      top = t;
+      sum *= f0;
+      v[0] *= f0, v[1] *= f0, v[2] *= f0, v[3] *= f0;
 #pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        float t = top[w];
-#pragma unroll
-        for (int k = 0; k < BATCH; ++k) t = fmaxf(t, m[w][k]);
-        const float f0 = top[w] == t ? 1.f : dev::ex2_approx(top[w] - t);
-        top[w] = t;
-        sum[w] *= f0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[w][e] *= f0;
-#pragma unroll
-        for (int k = 0; k < BATCH; ++k) {
-          const float f = m[w][k] == t ? 1.f : dev::ex2_approx(m[w][k] - t);
-          sum[w] += f * l[w][k];
-          v[w][0] += f * x[w][k].x, v[w][1] += f * x[w][k].y;
-          v[w][2] += f * x[w][k].z, v[w][3] += f * x[w][k].w;
-        }
+      for (int k = 0; k < kPagedJoin; ++k) {
+        const float f = m[k] == t ? 1.f : dev::ex2_approx(m[k] - t);
+        sum += f * l[k];
+        v[0] += f * x[k].x, v[1] += f * x[k].y, v[2] += f * x[k].z, v[3] += f * x[k].w;
       }
     }
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      const int idx = i0 + w * THREADS, n = idx / (D / 4), d = (idx - n * (D / 4)) * 4;
-      if (idx < work) paged_store<T, D>(p, b, head0 + n, d, v[w], top[w], sum[w]);
-    }
+    paged_store<T, D>(p, b, head0 + n, d, v, top, sum);
   }
 }
 
