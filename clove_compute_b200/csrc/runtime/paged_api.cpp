@@ -370,6 +370,7 @@ int clove_evict_cache(const clove_paged_cache* cache, float* key_weights, const 
   int rc = take_cache(cache, -1, &p.cache);
   if (rc) return rc;
   if (budget <= 0) return fail(CLOVE_ERR_INVALID_ARG, "budget must be positive");
+  if (budget > (1 << 30)) return fail(CLOVE_ERR_UNSUPPORTED, "budget beyond 2^30 tokens");
   if (recent < 0 || recent > budget) return fail(CLOVE_ERR_INVALID_ARG, "recent must be in [0, budget]");
   if (max_pages < 0 || dst_pages < 0) return fail(CLOVE_ERR_INVALID_ARG, "negative table width");
   if (static_cast<long long>(dst_pages) * cache->page_size < budget)

@@ -94,7 +94,7 @@ def test_attention_refusals(clove_lib, kw, code):
 @pytest.mark.parametrize("kw,code", [
     (dict(B=-1), 1), (dict(budget=0), 1), (dict(recent=-1), 1), (dict(recent=33), 1), (dict(dp=1), 1),
     (dict(mp=-1), 1), (dict(w=None), 1), (dict(dt=None), 1), (dict(kept=None), 1), (dict(nl=None), 1),
-    (dict(sl=None), 1), (dict(ts=3), 1), (dict(ds=3), 1), (dict(kept=A + 2), 1), (dict(mp=1 << 28, ts=1 << 28), 2),
+    (dict(sl=None), 1), (dict(ts=3), 1), (dict(ds=3), 1), (dict(kept=A + 2), 1), (dict(budget=(1 << 30) + 1, dp=1 << 27, ds=1 << 27), 2), (dict(mp=1 << 28, ts=1 << 28), 2),
 ])
 def test_evict_refusals(clove_lib, kw, code):
     assert _evict(clove_lib.lib(), _cache(), **kw) == code

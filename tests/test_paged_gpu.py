@@ -293,6 +293,124 @@ def test_attention_streams_and_graphs(clove_lib, cuda):
     assert clove_lib.device_error() == 0
 
 
+def test_attention_on_more_streams_than_are_kept(clove_lib, cuda):
+    """Each stream has a workspace of its own; beyond 64 streams a call brings one."""
+    from cuda.bindings import runtime as rt
+    g = _gen(12)
+    c, table, sl = _pages(clove_lib, [900, 17, 2500], 16, 2, 128, F16, "bshd", g)
+    Q = _randn((3, 8, 128), F16, g, 2.0)
+    want = clove_lib.paged_attention(Q, c, table, sl)
+    torch.cuda.synchronize()
+    handles = []
+    for _ in range(80):
+        err, s = rt.cudaStreamCreate()
+        assert int(err) == 0
+        handles.append(s)
+    try:
+        for _ in range(2):
+            got = [clove_lib.paged_attention(Q, c, table, sl, stream=int(s)) for s in handles]
+            torch.cuda.synchronize()
+            assert all(torch.equal(o, want) for o in got)
+    finally:
+        torch.cuda.synchronize()
+        for s in handles:
+            rt.cudaStreamDestroy(s)
+    assert clove_lib.device_error() == 0
+
+
+def test_attention_from_two_threads_on_one_stream(clove_lib, cuda):
+    import threading
+    g = _gen(13)
+    c, table, sl = _pages(clove_lib, [900, 17, 2500], 16, 2, 128, BF16, "bhsd", g)
+    Q = [_randn((3, 8, 128), BF16, g, 2.0) for _ in range(2)]
+    w = [torch.zeros((c.num_pages, 2, 16), device="cuda") for _ in range(2)]
+    want = []
+    for q, x in zip(Q, w):
+        want.append((clove_lib.paged_attention(q, c, table, sl, key_weights=x), x.clone()))
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        torch.cuda.set_device(0)
+        for _ in range(50):
+            o = clove_lib.paged_attention(Q[i], c, table, sl, key_weights=w[i])
+            if not torch.equal(o, want[i][0]):
+                bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    torch.cuda.synchronize()
+    assert not bad and all(torch.equal(x, y[1]) for x, y in zip(w, want))
+    assert clove_lib.device_error() == 0
+
+
+_CAPTURE_FIRST = r"""
+import torch
+import clove_compute_b200 as cc
+g = torch.Generator(device="cuda").manual_seed(1)
+K, V = (torch.randn((200, 16, 2, 128), device="cuda", generator=g).half() for _ in range(2))
+c = cc.PagedCache(K, V)
+table = torch.randperm(200, device="cuda", generator=g)[:190].to(torch.int32).view(1, 190)
+sl = torch.tensor([3000], dtype=torch.int32, device="cuda")
+Q = torch.randn((1, 8, 128), device="cuda", generator=g).half()
+torch.cuda.synchronize()
+gr = torch.cuda.CUDAGraph()
+with torch.cuda.graph(gr):
+    o = cc.paged_attention(Q, c, table, sl)
+for _ in range(3):
+    o.zero_()
+    gr.replay()
+    torch.cuda.synchronize()
+    first = o.clone()
+assert torch.equal(first, cc.paged_attention(Q, c, table, sl))
+assert cc.device_error() == 0
+print("captured first ok")
+"""
+
+
+def test_attention_captured_before_any_other_call(clove_lib, cuda):
+    """The first call of a process may be a captured one."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", _CAPTURE_FIRST], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured first ok" in r.stdout, r.stderr[-2000:]
+
+
+def test_attention_after_other_work_on_the_stream(clove_lib, cuda):
+    """Kernels overlap their predecessors' ends: a step whose queries, lengths and cache the
+    kernels just before it write, many times over, with nothing waiting in between."""
+    cc = clove_lib
+    g = _gen(14)
+    Hkv, H, D, ps, steps = 2, 8, 128, 16, 40
+    W = _randn((512, (H + 2 * Hkv) * D), F16, g, 512 ** -0.5)
+    X = _randn((steps, 2, 512), F16, g)
+    rope = cc.rope_table(256, D)
+    outs = []
+    for wait in (True, False):
+        K, V = (torch.zeros((12, ps, Hkv, D), dtype=F16, device="cuda") for _ in range(2))
+        cache = cc.PagedCache(K, V)
+        table = torch.arange(12, dtype=torch.int32, device="cuda").view(2, 6)
+        lens = torch.zeros(2, dtype=torch.int32, device="cuda")
+        got = []
+        for t in range(steps):
+            qkv = cc.gemm_fp16(X[t], W)
+            pos = lens.clone()
+            slots = table[:, t // ps] * ps + t % ps
+            lens += 1
+            q, k, v = (qkv[:, a * D:b * D].view(2, b - a, D) for a, b in ((0, H), (H, H + Hkv), (H + Hkv, H + 2 * Hkv)))
+            q, _ = cc.qk_norm_rope(q, k, rope, pos, V=v, cache=cache, slots=slots.to(torch.int32))
+            got.append(cc.paged_attention(q, cache, table, lens))
+            if wait:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        outs.append(torch.stack(got))
+    assert torch.equal(outs[0], outs[1])
+    assert cc.device_error() == 0
+
+
 # ---------------------------------------------------------------------------
 # norm + rotation + append
 # ---------------------------------------------------------------------------
