@@ -82,77 +82,92 @@ __global__ void __launch_bounds__(kEvictThreads, 1) evict_select_kernel(const Ev
   const int m = n - p.recent, want = p.budget - p.recent;
   const int per = (m + cs - 1) / cs;
   const int s0 = min(m, static_cast<int>(rank) * per), sn = min(m, s0 + per) - s0;
-  // Weights of keys of the slice, looked up for four keys at a time before any of them is
-  // read: first all pages (into the keys' places), then all weights. The loads are
-  // unconditional (index and page clamped, the result dropped), so that none waits for
-  // another; a bad page counts as weight 0. (Sixteen at a time take 3 us more on 4096 keys,
-  // fetching the instructions, and 0.6 us less on 131071.)
-  bool bad = false;
-  auto page_at = [&](int i) { return p.page_table[b * p.table_stride + ((s0 + i) >> p.cache.page_shift)]; };
+  for (int i = tid; i < kEvictBins; i += kEvictThreads) hist[0][i] = 0;
+  __syncthreads();
+  // Every warp keeps to a contiguous part [w0, w1) of the slice.
+  const int part = ((sn + kEvictWarps - 1) / kEvictWarps + 31) & ~31;
+  const int w0 = min(sn, warp * part), w1 = min(sn, w0 + part);
   auto good = [&](int pg) { return pg >= 0 && pg < p.cache.num_pages; };
+  auto page_at = [&](int i) { return p.page_table[b * p.table_stride + ((s0 + i) >> p.cache.page_shift)]; };
+  // (A clamped page: the load is unconditional, so that none waits for another.)
   auto weight_at = [&](int i, int pg) {
     return p.key_weights[((static_cast<long long>(good(pg) ? pg : 0) * p.cache.kv_heads + h)
                           << p.cache.page_shift) +
                          ((s0 + i) & page_mask)];
   };
-  for (int i = tid; i < kEvictBins; i += kEvictThreads) hist[0][i] = 0;
-  const int in_smem = LONG ? min(sn, kEvictCached) : sn;
-  constexpr int DEEP = 4;
-  for (int i0 = tid; i0 < in_smem; i0 += DEEP * kEvictThreads) {
-    int pg[DEEP];
-#pragma unroll
-    for (int k = 0; k < DEEP; ++k) pg[k] = page_at(min(i0 + k * kEvictThreads, in_smem - 1));
-#pragma unroll
-    for (int k = 0; k < DEEP; ++k)
-      if (i0 + k * kEvictThreads < in_smem) cached[i0 + k * kEvictThreads] = static_cast<uint32_t>(pg[k]);
-  }
-  for (int i0 = tid; i0 < in_smem; i0 += DEEP * kEvictThreads) {
-    int pg[DEEP];
-    float w[DEEP];
-#pragma unroll
-    for (int k = 0; k < DEEP; ++k) {  // (only this thread's own places hold pages still)
-      const int i = i0 + k * kEvictThreads;
-      pg[k] = static_cast<int>(cached[i < in_smem ? i : i0]);
-    }
-#pragma unroll
-    for (int k = 0; k < DEEP; ++k) w[k] = weight_at(min(i0 + k * kEvictThreads, in_smem - 1), pg[k]);
-#pragma unroll
-    for (int k = 0; k < DEEP; ++k) {
-      if (i0 + k * kEvictThreads < in_smem) cached[i0 + k * kEvictThreads] = weight_order(good(pg[k]) ? w[k] : 0.f);
-      bad = bad || !good(pg[k]);
-    }
-  }
-  if (bad) dev::record_error(dev::kDevErrBadIndex);
-  __syncthreads();
+  bool bad = false;
   auto key = [&](int i) {
-    if (!LONG || i < in_smem) return cached[i];
+    if (!LONG || i < kEvictCached) return cached[i];
     const int pg = page_at(i);
     const float w = weight_at(i, pg);
-    if (!good(pg)) dev::record_error(dev::kDevErrBadIndex);
-    return weight_order(good(pg) ? w : 0.f);
+    bad = bad || !good(pg);
+    return weight_order(good(pg) ? w : 0.f);  // a bad page counts as weight 0
   };
-
-  uint32_t prefix = 0;  // digits chosen so far
-  uint32_t left = static_cast<uint32_t>(want);
-  for (int d = 0; d < 3; ++d) {
-    const int shift = d == 0 ? 21 : d == 1 ? 10 : 0, bits = d == 2 ? 10 : 11;
-    const uint32_t mask = (1u << bits) - 1u;
-    uint32_t* mine = hist[d & 1];
-#pragma unroll 4
-    for (int base = 0; base < sn; base += kEvictThreads) {
-      const int i = base + tid;
-      const uint32_t u = i < sn ? key(i) : 0u;
-      const bool in = i < sn && (d == 0 || (u >> (shift + bits)) == prefix);
-      const uint32_t digit = (u >> shift) & mask;
-      // The first lane's digit is counted once for the warp: equal weights (zeros, as a
-      // rule) would otherwise queue up at one address.
-      const unsigned act = __ballot_sync(0xffffffffu, in);
-      if (act == 0u) continue;
+  // One more key with this digit, for the lanes with `in`. Where many lanes have one, the
+  // first lane's digit is counted once for the warp: equal weights (zeros, as a rule) would
+  // otherwise queue up at one address.
+  auto count = [&](uint32_t* mine, bool in, uint32_t digit) {
+    const unsigned act = __ballot_sync(0xffffffffu, in);
+    if (__popc(act) > 4) {
       const int lead = __ffs(act) - 1;
       const uint32_t d0 = __shfl_sync(0xffffffffu, digit, lead);
       const unsigned same = __ballot_sync(0xffffffffu, in && digit == d0);
       if (lane == lead) atomicAdd(&mine[d0], static_cast<uint32_t>(__popc(same)));
-      else if (in && digit != d0) atomicAdd(&mine[digit], 1u);
+      in = in && digit != d0;
+    }
+    if (in) atomicAdd(&mine[digit], 1u);
+  };
+  // The weights: 256 keys at a time, whose pages (of 16 keys or more: at most 17) one load
+  // of the warp brings, the next 256 keys' pages ahead of their use. The first digit is
+  // counted as they arrive.
+  const bool wide = p.cache.page_shift >= 4;
+  auto pages_of = [&](int base) {
+    const int first = (s0 + base) >> p.cache.page_shift, last = (s0 + min(base + 256, w1) - 1) >> p.cache.page_shift;
+    return wide && base < w1 ? p.page_table[b * p.table_stride + min(first + lane, last)] : 0;
+  };
+  int win = pages_of(w0);
+#pragma unroll 1
+  for (int base = w0; base < w1; base += 256) {
+    const int now = win, first = (s0 + base) >> p.cache.page_shift;
+    win = pages_of(base + 256);
+    float w[8];
+    int pg[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int i = min(base + 32 * k + lane, w1 - 1);
+      pg[k] = __shfl_sync(0xffffffffu, now, (((s0 + i) >> p.cache.page_shift) - first) & 31);
+      if (!wide) pg[k] = page_at(i);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w[k] = weight_at(min(base + 32 * k + lane, w1 - 1), pg[k]);
+    const int n8 = min(8, (w1 - base + 31) / 32);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int i = base + 32 * k + lane;
+      if (k >= n8) break;
+      bad = bad || (i < w1 && !good(pg[k]));
+      const uint32_t u = weight_order(good(pg[k]) ? w[k] : 0.f);
+      if (i < w1 && (!LONG || i < kEvictCached)) cached[i] = u;
+      count(hist[0], i < w1, u >> 21);
+    }
+  }
+  __syncwarp();
+
+  uint32_t prefix = 0;  // digits chosen so far
+  uint32_t left = static_cast<uint32_t>(want);
+#pragma unroll 1
+  for (int d = 0; d < 3; ++d) {
+    const int shift = d == 0 ? 21 : d == 1 ? 10 : 0, bits = d == 2 ? 10 : 11;
+    const uint32_t mask = (1u << bits) - 1u;
+    uint32_t* mine = hist[d & 1];
+    if (d > 0) {
+#pragma unroll 2
+      for (int base = w0; base < w1; base += 32) {
+        const int i = base + lane;
+        const uint32_t u = i < w1 ? key(i) : 0u;
+        const bool in = i < w1 && (u >> (shift + bits)) == prefix;
+        if (__any_sync(0xffffffffu, in)) count(mine, in, (u >> shift) & mask);
+      }
     }
     __syncthreads();
     // Sums of 64 bins each, one per warp, from the largest down.
@@ -210,11 +225,10 @@ __global__ void __launch_bounds__(kEvictThreads, 1) evict_select_kernel(const Ev
     prefix = (prefix << bits) | pick[0];
     __syncthreads();
   }
-  // Keys above and equal to the threshold in each warp's contiguous part.
-  const int part = ((sn + kEvictWarps - 1) / kEvictWarps + 31) & ~31;
-  const int w0 = min(sn, warp * part), w1 = min(sn, w0 + part);
+  if (bad) dev::record_error(dev::kDevErrBadIndex);
+  // Keys above and equal to the threshold in each warp's part.
   uint32_t gt_n = 0, eq_n = 0;
-#pragma unroll 4
+#pragma unroll 2
   for (int i = w0 + lane; i < w1; i += 32) {
     const uint32_t u = key(i);
     gt_n += u > prefix ? 1u : 0u;
@@ -239,29 +253,52 @@ __global__ void __launch_bounds__(kEvictThreads, 1) evict_select_kernel(const Ev
   dev::cluster_sync_all();
   // `left` keys equal to the threshold are kept, the first ones. What the slices, and the
   // warps' parts, before this one keep:
+  // (Lanes 0 .. rank - 1 hold the slices', then lanes 0 .. warp - 1 the parts' counts.)
   uint32_t eq_before = 0, out = 0;
-  for (uint32_t r = 0; r < rank; ++r) {
-    const uint32_t gt = ld_cluster_u32(&counts[0], r), eq = ld_cluster_u32(&counts[1], r);
-    out += gt + min(eq, left - min(left, eq_before));
-    eq_before += eq;
-  }
-  for (int w = 0; w < warp; ++w) {
-    out += warp_a[w] + min(warp_b[w], left - min(left, eq_before));
-    eq_before += warp_b[w];
-  }
+  auto skip = [&](uint32_t gt, uint32_t eq) {
+    uint32_t inc = eq;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    const uint32_t before = eq_before + inc - eq;
+    uint32_t kept_n = gt + min(eq, left - min(left, before));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) kept_n += __shfl_xor_sync(0xffffffffu, kept_n, o);
+    out += kept_n;
+    eq_before += __shfl_sync(0xffffffffu, inc, 31);
+  };
+  const bool slice_before = lane < static_cast<int>(rank);
+  skip(slice_before ? ld_cluster_u32(&counts[0], lane) : 0u, slice_before ? ld_cluster_u32(&counts[1], lane) : 0u);
+  skip(lane < warp ? warp_a[lane] : 0u, lane < warp ? warp_b[lane] : 0u);
   dev::cluster_arrive();  // no CTA leaves while its counts may be read
   const unsigned below = (1u << lane) - 1u;
-#pragma unroll 4
-  for (int base = w0; base < w1; base += 32) {
-    const int i = base + lane;
-    const uint32_t u = i < w1 ? key(i) : 0u;
-    const bool eq = i < w1 && u == prefix;
-    const unsigned eq_b = __ballot_sync(0xffffffffu, eq);
-    const bool take = (i < w1 && u > prefix) || (eq && eq_before + __popc(eq_b & below) < left);
-    const unsigned tk = __ballot_sync(0xffffffffu, take);
-    if (take) kept[out + __popc(tk & below)] = s0 + i;
-    out += __popc(tk);
-    eq_before += __popc(eq_b);
+  if (eq_n == 0 || eq_before >= left || eq_before + eq_n <= left) {
+    // All of the part's equal keys are kept, or none: one comparison decides.
+    const bool with_eq = eq_before < left;
+#pragma unroll 2
+    for (int base = w0; base < w1; base += 32) {
+      const int i = base + lane;
+      const uint32_t u = i < w1 ? key(i) : 0u;
+      const bool take = i < w1 && (with_eq ? u >= prefix : u > prefix);
+      const unsigned tk = __ballot_sync(0xffffffffu, take);
+      if (take) kept[out + __popc(tk & below)] = s0 + i;
+      out += __popc(tk);
+    }
+  } else {
+#pragma unroll 1
+    for (int base = w0; base < w1; base += 32) {
+      const int i = base + lane;
+      const uint32_t u = i < w1 ? key(i) : 0u;
+      const bool eq = i < w1 && u == prefix;
+      const unsigned eq_b = __ballot_sync(0xffffffffu, eq);
+      const bool take = (i < w1 && u > prefix) || (eq && eq_before + __popc(eq_b & below) < left);
+      const unsigned tk = __ballot_sync(0xffffffffu, take);
+      if (take) kept[out + __popc(tk & below)] = s0 + i;
+      out += __popc(tk);
+      eq_before += __popc(eq_b);
+    }
   }
   // The recent keys.
   for (int j = static_cast<int>(rank) * kEvictThreads + tid; j < p.recent; j += cs * kEvictThreads)
