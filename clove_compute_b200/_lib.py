@@ -112,19 +112,12 @@ def check(rc: int) -> None:
         raise CloveError(rc, msg)
 
 
-_fast = None
-
-
 def fastcall():
-    """The CPython entry points of the paged-cache operators (``csrc/binding/fastcall.c``),
-    bound to the loaded library. Raises if they were not built."""
-    global _fast
-    if _fast is None:
-        lib()
-        try:
-            from . import _fastcall
-        except ImportError as e:
-            raise ImportError("_fastcall.so is missing: build it with `python -m clove_compute_b200.build`") from e
-        _fastcall.init(_LIB_PATH)
-        _fast = _fastcall
-    return _fast
+    """The CPython entry points of the paged-cache operators (``csrc/binding/fastcall.c``).
+    Raises if they were not built."""
+    lib()
+    try:
+        from . import _fastcall
+    except ImportError as e:
+        raise ImportError("_fastcall.so is missing: build it with `python -m clove_compute_b200.build`") from e
+    return _fastcall

@@ -711,6 +711,95 @@ def test_evict_capture(clove_lib, cuda):
 
 
 # ---------------------------------------------------------------------------
+# refusals of the Python layer (nothing is launched)
+# ---------------------------------------------------------------------------
+def _call_args(cc):
+    K, V = (torch.zeros((8, 16, 2, 128), dtype=F16, device="cuda") for _ in range(2))
+    cache = cc.PagedCache(K, V)
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")
+    f32 = lambda *s: torch.zeros(s, device="cuda")
+    h = lambda *s: torch.zeros(s, dtype=F16, device="cuda")
+    rope = dict(Q=h(3, 4, 128), K=h(3, 2, 128), rope_table=f32(64, 128), positions=i32(3), q_weight=h(128),
+                k_weight=h(128), V=h(3, 2, 128), cache=cache, slots=i32(3) - 1)
+    attn = dict(Q=h(3, 4, 128), cache=cache, page_table=i32(3, 2), seq_lens=i32(3), lse=f32(3, 4),
+                key_weights=f32(8, 2, 16), O=h(3, 4, 128))
+    evict = dict(cache=cache, key_weights=f32(8, 2, 16), page_table=i32(3, 2), seq_lens=i32(3),
+                 dst_table=i32(3, 2), budget=20)
+    return {"qk_norm_rope": rope, "paged_attention": attn, "evict_cache": evict}
+
+
+def _wrongs(name, x):
+    """Wrong values for a tensor argument and the exceptions they may raise."""
+    yield x.cpu(), ValueError
+    yield x.double(), TypeError
+    yield None, (TypeError, ValueError)
+    yield "text", TypeError
+    yield torch.cat([x, x]), ValueError               # another first size
+    yield x[..., :-1], ValueError                     # another last size
+    yield x.unsqueeze(0), ValueError                  # another number of dimensions
+    wide = torch.zeros(x.shape[:-1] + (2 * x.shape[-1],), dtype=x.dtype, device="cuda")
+    yield wide[..., ::2], ValueError                  # a stride in the last dimension
+
+
+@pytest.mark.parametrize("fn", ["qk_norm_rope", "paged_attention", "evict_cache"])
+def test_python_layer_refuses(clove_lib, cuda, fn):
+    args = _call_args(clove_lib)[fn]
+    call = getattr(clove_lib, fn)
+    call(**args)  # as it stands it runs
+    may_differ = {("rope_table", 0), ("page_table", 1), ("dst_table", 1)}  # sizes that are the caller's choice
+    optional = {"lse", "key_weights", "O"} if fn == "paged_attention" else set()
+    for name, x in args.items():
+        if not isinstance(x, torch.Tensor):
+            continue
+        for k, (bad, exc) in enumerate(_wrongs(name, x)):
+            if (k == 4 and (name, 0) in may_differ) or (k == 5 and (name, 1) in may_differ):
+                continue
+            if k == 2 and name in optional:
+                continue
+            with pytest.raises(exc):
+                call(**{**args, name: bad})
+    with pytest.raises(TypeError):
+        call(**{**args, "cache": "text"})
+    if fn == "qk_norm_rope":
+        for a in (dict(cache=None), dict(V=None, slots=None), dict(q_weight=None), dict(eps="x")):
+            with pytest.raises((TypeError, ValueError)):
+                call(**{**args, **a})
+        with pytest.raises(clove_lib.CloveError):
+            call(**{**args, "eps": -1.0})
+    elif fn == "paged_attention":
+        for a in (dict(key_weights=None, accumulate=True), dict(window="x"), dict(window=1 << 40), dict(scale="x")):
+            with pytest.raises((TypeError, ValueError)):
+                call(**{**args, **a})
+        with pytest.raises(clove_lib.CloveError):
+            call(**{**args, "scale": 0.0})
+    else:
+        for a in (dict(budget=0), dict(budget=1 << 40), dict(recent="x")):
+            with pytest.raises((TypeError, ValueError)):
+                call(**{**args, **a})
+        for a in (dict(recent=21), dict(budget=100)):
+            with pytest.raises(clove_lib.CloveError):
+                call(**{**args, **a})
+    torch.cuda.synchronize()
+    assert clove_lib.device_error() == 0
+
+
+def test_python_layer_keeps_no_references(clove_lib, cuda):
+    """Calls, refused ones too, leave their arguments' and results' reference counts alone."""
+    import sys
+    for fn, args in _call_args(clove_lib).items():
+        call = getattr(clove_lib, fn)
+        before = {n: sys.getrefcount(x) for n, x in args.items()}
+        for _ in range(50):
+            r = call(**args)
+            with pytest.raises((TypeError, ValueError)):
+                call(**{**args, "page_table" if fn != "qk_norm_rope" else "positions": None})
+        fresh = [x for x in (r if isinstance(r, tuple) else (r,)) if x is not None and not any(x is y for y in args.values())]
+        assert all(sys.getrefcount(x) <= 5 for x in fresh)
+        del r, fresh
+        assert {n: sys.getrefcount(x) for n, x in args.items()} == before
+
+
+# ---------------------------------------------------------------------------
 # together, as a decode loop uses them
 # ---------------------------------------------------------------------------
 def test_decode_loop_agrees_with_prefill_attention(clove_lib, cuda):
