@@ -117,36 +117,41 @@ __global__ void __launch_bounds__(kEvictThreads, 1) evict_select_kernel(const Ev
     }
     if (in) atomicAdd(&mine[digit], 1u);
   };
-  // The weights: 256 keys at a time, whose pages (of 16 keys or more: at most 17) one load
-  // of the warp brings, the next 256 keys' pages ahead of their use. The first digit is
+  // The weights: KEYS at a time, whose pages (of 16 keys or more: fewer than 32) one load of
+  // the warp brings, the next KEYS' pages ahead of their use. The first digit is
   // counted as they arrive.
+  constexpr int DEEP = 4, KEYS = 32 * DEEP;
   const bool wide = p.cache.page_shift >= 4;
   auto pages_of = [&](int base) {
-    const int first = (s0 + base) >> p.cache.page_shift, last = (s0 + min(base + 256, w1) - 1) >> p.cache.page_shift;
+    const int first = (s0 + base) >> p.cache.page_shift, last = (s0 + min(base + KEYS, w1) - 1) >> p.cache.page_shift;
     return wide && base < w1 ? p.page_table[b * p.table_stride + min(first + lane, last)] : 0;
   };
   int win = pages_of(w0);
 #pragma unroll 1
-  for (int base = w0; base < w1; base += 256) {
+  for (int base = w0; base < w1; base += KEYS) {
     const int now = win, first = (s0 + base) >> p.cache.page_shift;
-    win = pages_of(base + 256);
-    float w[8];
-    int pg[8];
+    win = pages_of(base + KEYS);
+    float w[DEEP];
+    int pg[DEEP];
+    uint32_t ok = 0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < DEEP; ++k) {
       const int i = min(base + 32 * k + lane, w1 - 1);
       pg[k] = __shfl_sync(0xffffffffu, now, (((s0 + i) >> p.cache.page_shift) - first) & 31);
       if (!wide) pg[k] = page_at(i);
     }
 #pragma unroll
-    for (int k = 0; k < 8; ++k) w[k] = weight_at(min(base + 32 * k + lane, w1 - 1), pg[k]);
-    const int n8 = min(8, (w1 - base + 31) / 32);
+    for (int k = 0; k < DEEP; ++k) {
+      ok |= good(pg[k]) ? 1u << k : 0u;
+      w[k] = weight_at(min(base + 32 * k + lane, w1 - 1), pg[k]);
+    }
+    bad = bad || ok != (1u << DEEP) - 1u;  // (places past the end repeat the last key's)
+    const int n8 = min(DEEP, (w1 - base + 31) / 32);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < DEEP; ++k) {
       const int i = base + 32 * k + lane;
       if (k >= n8) break;
-      bad = bad || (i < w1 && !good(pg[k]));
-      const uint32_t u = weight_order(good(pg[k]) ? w[k] : 0.f);
+      const uint32_t u = weight_order(ok & (1u << k) ? w[k] : 0.f);
       if (i < w1 && (!LONG || i < kEvictCached)) cached[i] = u;
       count(hist[0], i < w1, u >> 21);
     }
@@ -426,7 +431,8 @@ int launch_evict_cache(const kern::EvictParams& p, const DeviceInfo& dev, cudaSt
   }
   // CTAs per (sequence, head): up to 8 while all of them fit on the GPU at once (one per
   // SM) and each has 4096 keys, four per thread. (Clusters of 16 do not all fit: 131071 keys
-  // of 8 heads take 56 us with them, 42 us with 8.)
+  // of 8 heads take 56 us with them, 42 us with 8. Twice as many CTAs as SMs: 8 sequences of
+  // 32768 keys, 8 heads, ragged 82 -> 76 us, but of equal lengths 125 -> 134 us.)
   const long long rows = static_cast<long long>(p.batch) * p.cache.kv_heads;
   int cs = 1;
   while (cs < 8 && rows * cs * 2 <= dev.num_sms && p.capacity > cs * 4 * kern::kEvictThreads) cs *= 2;
