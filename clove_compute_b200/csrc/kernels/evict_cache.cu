@@ -182,11 +182,11 @@ __global__ void __launch_bounds__(kEvictThreads, 1) evict_select_kernel(const Ev
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
       if (lane == 0) coarse[d & 1][warp] = v;
-      hist[(d & 1) ^ 1][bin] = hist[(d & 1) ^ 1][bin + 1] = 0;  // for the next digit
     }
     // All CTAs' histograms of this digit are complete, and those of the digit before have
-    // been read. (The other histogram was read before the last barrier: it may be cleared.)
+    // been read by all of them: only now may this one's be cleared, for the next digit.
     dev::cluster_sync_all();
+    for (int i = tid; i < kEvictBins; i += kEvictThreads) hist[(d & 1) ^ 1][i] = 0;
     if (warp == 0) {
       // Warp 0 finds the `left`-th largest key's 64 bins, then its bin, adding up the CTAs'
       // counts of those alone.

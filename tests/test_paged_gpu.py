@@ -661,6 +661,27 @@ def test_evict_long_sequence(clove_lib, cuda, n, Hkv, budget, recent, kind):
     _check_evict(clove_lib, [n], budget, recent, 64, Hkv, 64, E4M3, "bshd", kind)
 
 
+def test_evict_repeats_bit_for_bit(clove_lib, cuda):
+    """Clusters of eight CTAs that run beside each other at different speeds (other rows end
+    at once, another stream is busy): every run keeps the same keys."""
+    g = _gen(31)
+    lens = [60001, 0, 40, 33000]
+    cache, table, sl = _pages(clove_lib, lens, 32, 2, 64, E4M3, "bhsd", g, spare=4 * 100)
+    used = set(table[table >= 0].tolist())
+    free = [pg for pg in range(cache.num_pages) if pg not in used]
+    dst = torch.tensor([free[i * 94:(i + 1) * 94] for i in range(4)], dtype=torch.int32, device="cuda")
+    sets = [_weights(kind, (cache.num_pages, 2, 32), g) for kind in ("zeros", "ties", "odd", "random")]
+    want = [clove_lib.evict_cache(cache, w, table, sl, dst, 3000, 17)[0].clone() for w in sets]
+    torch.cuda.synchronize()
+    other, x = torch.cuda.Stream(), torch.randn(1 << 24, device="cuda")
+    for i in range(200):
+        with torch.cuda.stream(other):
+            x.mul_(1.0)
+        got, _ = clove_lib.evict_cache(cache, sets[i % 4], table, sl, dst, 3000, 17)
+        assert torch.equal(got, want[i % 4]), i
+    torch.cuda.synchronize()
+
+
 def test_evict_long_rows_in_one_cta(clove_lib, cuda):
     """Over 148 rows: one CTA each, with slices longer than its shared memory holds."""
     _check_evict(clove_lib, [30011], 5000, 100, 64, 150, 64, E4M3, "bhsd", "zeros")
