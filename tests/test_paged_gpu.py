@@ -134,6 +134,36 @@ def test_attention_work_split(clove_lib, cuda, lens):
     _check_attention(clove_lib, c, table, sl, _randn((len(lens), 8, 64), F16, g, 2.0))
 
 
+@pytest.mark.parametrize("lens,D,cache,G,weights", [
+    ([300007, 0, 151001, 41], 64, E4M3, 3, True),
+    ([200003, 40, 60000], 128, F16, 4, False),
+    ([131071, 131072, 5], 128, E4M3, 12, False),
+    ([130001], 256, BF16, 2, False),
+])
+def test_attention_long_calls(clove_lib, cuda, lens, D, cache, G, weights):
+    """Hundreds of tiles for every CTA, items over dozens of CTAs, page windows refilled many
+    times: right, the same bit for bit every time, and captured."""
+    g = _gen(D + G)
+    Hkv = 8
+    s = 0.5 if cache == E4M3 else 1.0
+    dtype = F16 if cache == E4M3 else cache
+    c, table, sl = _pages(clove_lib, lens, 64, Hkv, D, cache, "bshd", g, k_scale=s, v_scale=s)
+    Q = _randn((len(lens), Hkv * G, D), dtype, g, 2.0)
+    w = torch.zeros((c.num_pages, Hkv, 64), device="cuda") if weights else None
+    want = _check_attention(clove_lib, c, table, sl, Q, key_weights=w, before=torch.zeros_like(w) if weights else None)
+    for _ in range(10):
+        assert torch.equal(clove_lib.paged_attention(Q, c, table, sl), want)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        o = clove_lib.paged_attention(Q, c, table, sl)
+    for _ in range(3):
+        o.zero_()
+        gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, want)
+    assert clove_lib.device_error() == 0
+
+
 @pytest.mark.parametrize("window", [1, 15, 16, 17, 100, 4096])
 @pytest.mark.parametrize("ps", [4, 32])
 def test_attention_window_skips_released_pages(clove_lib, cuda, window, ps):
