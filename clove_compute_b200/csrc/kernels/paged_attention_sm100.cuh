@@ -27,6 +27,12 @@
 //   is rounded; scores, maxima, totals and O stay in fp32.
 // * Softmax. Running maximum and total per warp; the maximum is reduced over the warp
 //   only when some lane's score exceeds it.
+//
+// Measured, back to back on one B200: 64 sequences of up to 16384 keys, 32 / 8 heads of 128,
+// fp16 162 us (6.4 TB/s, 0.97 of the copy rate); 2 x 131071 keys, 64 / 8 heads, e4m3 103 us
+// (0.79; rows of 128 bytes at strides of 1 KB; 96 us with a head's rows side by side); 1 x
+// 4096 keys, 32 / 32 heads, fp16 19 us, of which 9 read the cache, 4 pass before the first
+// key (length, page and key, three DRAM latencies in a row) and 4 in merging and joining.
 #pragma once
 
 #include <cuda_runtime.h>

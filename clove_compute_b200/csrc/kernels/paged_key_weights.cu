@@ -10,7 +10,9 @@ namespace clove {
 namespace kern {
 
 // Key weights from the stored scores: w_t = sum over the group of 2^(s_t - LSE2), written
-// to (or added to) the key's place in the paged weights. Reads 4 bytes per head and key.
+// to (or added to) the key's place in the paged weights. Reads 4 bytes per head and key, and
+// is bound by its few dependent loads: with the scores' stores it adds 8 us to 38 us of
+// attention (8 sequences of up to 20000 keys, 32 / 8 heads), 2 to 3 us to a small call.
 __global__ void __launch_bounds__(256) paged_key_weights_kernel(const PagedAttnParams p) {
   dev::grid_dependency_wait();
   const int page_mask = (1 << p.cache.page_shift) - 1;

@@ -300,7 +300,7 @@ int clove_paged_attention(const void* Q, long long q_stride, const clove_paged_c
                     o_stride < static_cast<long long>(num_heads) * D || table_stride < max_pages))
     return fail(CLOVE_ERR_INVALID_ARG, "a row stride is smaller than the row");
   const long long capacity = static_cast<long long>(max_pages) * cache->page_size;
-  if (capacity > INT_MAX - 4096) return fail(CLOVE_ERR_UNSUPPORTED, "page table rows name over 2^31 tokens");
+  if (capacity > INT_MAX - 65536) return fail(CLOVE_ERR_UNSUPPORTED, "page table rows name over 2^31 tokens");
   DeviceInfo dev;
   rc = current_device(&dev);
   if (rc) return rc;
