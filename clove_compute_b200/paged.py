@@ -40,11 +40,13 @@ class PagedCache:
                 raise ValueError(f"{n} must be 4-D, got shape {tuple(t.shape)}")
         if layout not in ("bshd", "bhsd"):
             raise ValueError("layout must be 'bshd' or 'bhsd'")
-        if K.shape != V.shape or K.dtype != V.dtype or K.device != V.device or K.stride() != V.stride():
+        # (The stride of a dimension of size 1 means nothing.)
+        strides, others = ([s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride())] for t in (K, V))
+        if K.shape != V.shape or K.dtype != V.dtype or K.device != V.device or strides != others:
             raise ValueError("K and V must agree in shape, strides, dtype and device")
         if K.numel() == 0:
             raise ValueError("the cache has no slots")
-        if K.stride(3) != 1:
+        if K.stride(3) != 1 or V.stride(3) != 1:
             raise ValueError("the last dimension of K and V must be contiguous")
         tok, head = (1, 2) if layout == "bshd" else (2, 1)
         self.K, self.V, self.layout = K, V, layout
@@ -53,8 +55,8 @@ class PagedCache:
         self.dtype, self.device, self.index = K.dtype, K.device, K.get_device()
         self.k_scale, self.v_scale = float(k_scale), float(v_scale)
         self.struct = PagedCacheStruct(K.data_ptr(), V.data_ptr(), self.num_pages, self.page_size,
-                                       self.num_kv_heads, self.head_dim, K.stride(0), K.stride(tok),
-                                       K.stride(head), DTYPES[K.dtype], self.k_scale, self.v_scale)
+                                       self.num_kv_heads, self.head_dim, strides[0], strides[tok],
+                                       strides[head], DTYPES[K.dtype], self.k_scale, self.v_scale)
         self._key = (ctypes.addressof(self.struct), self.index)
 
 

@@ -834,6 +834,31 @@ def test_python_layer_refuses(clove_lib, cuda, fn):
     assert clove_lib.device_error() == 0
 
 
+def test_empty_batches_and_single_dimensions(clove_lib, cuda):
+    """Calls of no sequence; caches whose dimensions of size 1 have odd strides."""
+    cc = clove_lib
+    g = _gen(40)
+    K, V = (torch.randn((9, 16, 1, 64), device="cuda", generator=g).half() for _ in range(2))
+    cache = cc.PagedCache(K, V)
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    tab = torch.zeros((0, 4), dtype=torch.int32, device="cuda")
+    assert cc.paged_attention(K.new_zeros((0, 3, 64)), cache, tab, none).shape == (0, 3, 64)
+    w = torch.zeros((9, 1, 16), device="cuda")
+    kept, new = cc.evict_cache(cache, w, tab, none, tab, 20)
+    assert kept.shape == (0, 1, 20) and new.shape == (0,)
+    table = torch.tensor([[3, 1, 8]], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([45], dtype=torch.int32, device="cuda")
+    Q = _randn((1, 3, 64), F16, g)
+    want = cc.paged_attention(Q, cache, table, lens)
+    odd = [t.as_strided(t.shape, (1024, 64, 7, 1)) for t in (K, V)]
+    assert torch.equal(cc.paged_attention(Q, cc.PagedCache(*odd), table, lens), want)
+    q1 = Q.as_strided((1, 3, 64), (13, 64, 1))
+    t1 = table.as_strided((1, 3), (-0, 1))
+    assert torch.equal(cc.paged_attention(q1, cache, t1, lens), want)
+    torch.cuda.synchronize()
+    assert cc.device_error() == 0
+
+
 def test_python_layer_keeps_no_references(clove_lib, cuda):
     """Calls, refused ones too, leave their arguments' and results' reference counts alone."""
     import sys
