@@ -23,8 +23,11 @@
 //   (or head elements) as the 16 rows and 8 query heads as the columns: a group of up to 8
 //   heads wastes nothing that costs time. (tcgen05 wants 64 or 128 rows of queries.)
 //   K and V reach the instructions by ldmatrix from XOR-swizzled rows; e4m3 elements are
-//   widened to fp16 in registers. P is passed as the sum of two 16-bit halves, so that no weight
-//   is rounded; scores, maxima, totals and O stay in fp32.
+//   widened to fp16 in registers. P is passed as the sum of two 16-bit halves: in bf16 they
+//   keep 2^-17 of a weight; in fp16, taken 2^15 times as large, 2^-23 of it, down to 2^-40 of
+//   the largest weight, below which weights vanish from the sum of values (unscaled halves
+//   lost what is below 2^-25: keys beside one that is 17 nats above them). Scores, maxima,
+//   totals and O stay in fp32.
 // * Softmax. Running maximum and total per warp; the maximum is reduced over the warp
 //   only when some lane's score exceeds it.
 //
@@ -295,6 +298,10 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
   // e4m3 elements (and their queries) are multiplied as fp16, whatever the query type.
   using MT = typename std::conditional<F8, __half, T>::type;
   using P2 = Pair<MT>;
+  // Weights are multiplied by this before they are halved (at most 32768 in fp16; the sums,
+  // at most 2^16 x 2^15 x 2^31 keys, stay far inside fp32), O by its inverse at the end.
+  // bf16 has fp32's exponents and needs none.
+  constexpr float P_UP = std::is_same<MT, __half>::value ? 32768.f : 1.f;
   constexpr int ROWB = S::ROWB, CPR = S::CPR, KK = D / 16, M = S::M;
   extern __shared__ __align__(1024) uint8_t smem[];
   float* merge = reinterpret_cast<float*>(smem + kPagedWarps * S::RING);
@@ -631,8 +638,8 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
             }
           }
       }
-      // P^T as the B operand: transposed 8 x 8 blocks of the score fragments; two 16-bit
-      // halves whose sum is p to fp32's precision (fp16: to 2^-25 of the largest weight).
+      // P^T as the B operand: transposed 8 x 8 blocks of the score fragments, as two 16-bit
+      // halves.
       uint32_t ph[M][NT][2], pl[M][NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -646,10 +653,11 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
             const float p1 = dev::ex2_approx(sc[g][nt][2 * e + 1] - mm1);
             l[nt][0] += p0;
             l[nt][1] += p1;
-            const uint32_t hi = P2::pack(p0, p1);
+            const float u0 = p0 * P_UP, u1 = p1 * P_UP;
+            const uint32_t hi = P2::pack(u0, u1);
             const float2 f = P2::unpack(hi);
             ph[g][nt][e] = transpose_8x8(hi);
-            pl[g][nt][e] = transpose_8x8(P2::pack(p0 - f.x, p1 - f.y));
+            pl[g][nt][e] = transpose_8x8(P2::pack(u0 - f.x, u1 - f.y));
           }
       }
       // O^T += V^T P^T: rows = head elements. 16-bit: tile kk holds elements 16 kk + row.
@@ -731,7 +739,7 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
         float top = sm_m[n];
 #pragma unroll
         for (int w = 1; w < kPagedWarps; ++w) top = fmaxf(top, sm_m[w * S::HEADS + n]);
-        const float f = m[nt][e] == top ? 1.f : dev::ex2_approx(m[nt][e] - top);
+        const float f = (m[nt][e] == top ? 1.f : dev::ex2_approx(m[nt][e] - top)) * (1.f / P_UP);
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) {
           const int d0 = kk * 16 + (F8 ? 2 * row4 : row4), d1 = d0 + (F8 ? 1 : 8);

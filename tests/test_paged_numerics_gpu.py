@@ -1,0 +1,79 @@
+"""Paged attention where the products' 16-bit operands could lose what fp32 keeps, against
+plain 64-bit statements (tests/paged_ref.py)."""
+import math
+
+import pytest
+import torch
+
+from tests import paged_ref as ref
+
+pytestmark = pytest.mark.gpu
+F16, BF16, E4M3 = torch.float16, torch.bfloat16, torch.float8_e4m3fn
+
+
+def _bound(q, k, v, scale, products):
+    """(o, lse, bounds of both before o's rounding) as paged_ref.attention, but with the
+    weights' own rounding: two halves leave 2^-17 (bf16) or 2^-23 (fp16) of each, and fp16
+    halves of weights that are passed 2^15 times as large end at 2^-25, which is 2^-40 of a
+    largest weight."""
+    H, D = q.shape
+    n, Hkv = k.shape[0], k.shape[1]
+    o, lse, _, _, b_lse, _ = ref.attention(q, k, v, scale, 0)
+    qg = q.double().view(Hkv, H // Hkv, D)
+    s = torch.einsum("hgd,thd->hgt", qg, k) * scale
+    mag = torch.einsum("hgd,thd->hgt", qg.abs(), k.abs()) * scale
+    p = torch.exp(s - torch.logsumexp(s, -1, keepdim=True))
+    e_s = (D / 16 + 16) * 2 * ref.U * mag.amax(-1) + 8 * ref.U * s.abs().amax(-1) + 4 * ref.U
+    steps = (n / 64 + 64) * 2 * ref.U
+    size = torch.einsum("hgt,thd->hgd", p, v.abs())
+    rel, floor = (2.0 ** -17, 0.0) if products == BF16 else (2.0 ** -23, 2.0 ** -40)
+    b = size * (2 * e_s + 2 * steps + rel)[..., None] + floor * p.amax(-1, keepdim=True) * v.abs().sum(0)[:, None, :]
+    return o, lse, b.reshape(H, D), b_lse
+
+
+def _cache_and_table(cc, K, V, lens, k_scale=1.0, v_scale=1.0):
+    """Contiguous rows [sum of lens, Hkv, D] (each a multiple of 16) as pages of 16."""
+    shape = (K.shape[0] // 16, 16) + tuple(K.shape[1:])
+    cache = cc.PagedCache(K.view(shape), V.view(shape), k_scale=k_scale, v_scale=v_scale)
+    table = torch.zeros((len(lens), max(lens) // 16), dtype=torch.int32, device="cuda")
+    first = 0
+    for i, n in enumerate(lens):
+        table[i, :n // 16] = torch.arange(first // 16, (first + n) // 16, device="cuda")
+        first += n
+    return cache, table, torch.tensor(lens, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("dtype,cache_dtype,D,G", [
+    (F16, F16, 128, 4), (F16, F16, 64, 1), (F16, F16, 256, 2), (F16, F16, 128, 16),
+    (F16, E4M3, 128, 4), (BF16, E4M3, 128, 8), (BF16, E4M3, 64, 3), (BF16, BF16, 128, 4),
+])
+@pytest.mark.parametrize("gap", [12.0, 15.5, 17.0, 18.5, 22.0])
+def test_attention_with_a_dominant_key(clove_lib, cuda, dtype, cache_dtype, D, G, gap):
+    """One key of each sequence has a score `gap` nats above all the others and a value of
+    zero: the output is the others' alone, each of weight e^-gap (2^-17 to 2^-32). Enough
+    sequences that a warp has thousands of keys beside it; at the start, in the middle and
+    at the end."""
+    g = torch.Generator(device="cuda").manual_seed(int(gap * 10) + D + G)
+    B, Hkv, n = 40, 8, 2048
+    scale = D ** -0.5
+    Q = (0.1 * torch.randn((B, Hkv * G, D), device="cuda", generator=g)).to(dtype)
+    Q[..., 0] = 8.0
+    K = 0.1 * torch.randn((B * n, Hkv, D), device="cuda", generator=g)
+    V = 1.0 + 0.25 * torch.randn((B * n, Hkv, D), device="cuda", generator=g)
+    K[..., 0] = 0.0
+    at = torch.tensor([b * n + (0, n // 2, n - 1)[b % 3] for b in range(B)], device="cuda")
+    K[at, :, 0] = gap / (8.0 * scale)
+    V[at] = 0.0
+    K, V = K.to(cache_dtype), V.to(cache_dtype)
+    cache, table, lens = _cache_and_table(clove_lib, K, V, [n] * B)
+    lse = torch.empty((B, Hkv * G), device="cuda")
+    O = clove_lib.paged_attention(Q, cache, table, lens, lse=lse)
+    torch.cuda.synchronize()
+    assert clove_lib.device_error() == 0
+    products = BF16 if cache_dtype == BF16 else F16
+    for b in range(B):
+        k, v = (ref.rows(c, "bshd", table[b], n, 16) for c in (cache.K, cache.V))
+        o, l, b_o, b_l = _bound(Q[b], k, v, scale, products)
+        err, tol = (O[b].double() - o).abs(), b_o + ref.half_step(o.abs() + b_o, dtype)
+        assert torch.all(err <= tol), (b, float((err / tol).max()), float((err / o.abs().clamp(min=1e-30)).max()))
+        assert torch.all((lse[b].double() - l).abs() <= b_l)
