@@ -491,8 +491,9 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
   };
   auto scale_q = [&]() {
     // bf16 queries as fp16: each head's row is first multiplied by the power of two that
-    // brings its largest element to [1, 2) (exact; elements below 2^-24 of the largest
-    // vanish, as they would in the fp32 sum), its scores by the inverse.
+    // brings its largest element to [2^15, 2^16), its scores by the inverse. Elements down to
+    // 2^-32 of the largest keep all their bits, smaller ones end at 2^-40 of it. (Products
+    // with e4m3 stay below 2^25, far inside the fp32 sum.)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       uint32_t big = 0u;
@@ -503,17 +504,19 @@ __global__ void __launch_bounds__(PagedShape<F8, D, NT>::THREADS,
           big = max(big, max(qf[nt][kk][e] & 0x7fff0000u, (qf[nt][kk][e] << 16) & 0x7fff0000u));
       big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
       big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
-      uint32_t ex = big >> 23;  // biased exponent; zero rows, infinities and NaN unscaled
-      ex = ex == 0u || ex == 255u ? 127u : min(ex, 253u);
-      const float down = __uint_as_float((254u - ex) << 23);
+      // Biased exponent; rows below 2^-111 are multiplied by 2^126, those with an infinity or
+      // NaN by 1.
+      uint32_t ex = big >> 23;
+      ex = ex == 255u ? 142u : max(ex, 16u);
+      const float scale_up = __uint_as_float((269u - ex) << 23);
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float2 f = Pair<__nv_bfloat16>::unpack(qf[nt][kk][e]);
-          qf[nt][kk][e] = P2::pack(f.x * down, f.y * down);
+          qf[nt][kk][e] = P2::pack(f.x * scale_up, f.y * scale_up);
         }
-      const float up = __uint_as_float(ex << 23) * p.scale_log2;
+      const float up = __uint_as_float((ex - 15u) << 23) * p.scale_log2;
       q_scale[nt][0] = __shfl_sync(0xffffffffu, up, col4 * 8);
       q_scale[nt][1] = __shfl_sync(0xffffffffu, up, col4 * 8 + 4);
     }

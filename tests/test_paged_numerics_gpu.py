@@ -77,3 +77,32 @@ def test_attention_with_a_dominant_key(clove_lib, cuda, dtype, cache_dtype, D, G
         err, tol = (O[b].double() - o).abs(), b_o + ref.half_step(o.abs() + b_o, dtype)
         assert torch.all(err <= tol), (b, float((err / tol).max()), float((err / o.abs().clamp(min=1e-30)).max()))
         assert torch.all((lse[b].double() - l).abs() <= b_l)
+
+
+@pytest.mark.parametrize("D,G", [(64, 3), (128, 4), (128, 16), (256, 2)])
+@pytest.mark.parametrize("small", [2.0 ** -12, 2.0 ** -17, 2.0 ** -20, 2.0 ** -24])
+def test_attention_bf16_queries_of_wide_range(clove_lib, cuda, D, G, small):
+    """bf16 query rows over an e4m3 cache, one element `1 / small` times as large as the
+    others, on which every key is zero: the scores are made of the small elements alone."""
+    g = torch.Generator(device="cuda").manual_seed(D + G)
+    lens, Hkv = [512, 96, 16], 2
+    n = sum(lens)
+    for top in (1.0, 2.0 ** -100, 2.0 ** 90):
+        Q = (torch.randn((3, Hkv * G, D), device="cuda", generator=g) * small).clamp(-3 * small, 3 * small)
+        Q[..., 5] = 1.0
+        Q = (Q * top).to(BF16)
+        K = torch.randn((n, Hkv, D), device="cuda", generator=g) * 2
+        K[..., 5] = 0.0
+        V = torch.randn((n, Hkv, D), device="cuda", generator=g)
+        scale = D ** -0.5 / (small * top)
+        cache, table, sl = _cache_and_table(clove_lib, K.to(E4M3), V.to(E4M3), lens)
+        lse = torch.empty((3, Hkv * G), device="cuda")
+        O = clove_lib.paged_attention(Q, cache, table, sl, scale=scale, lse=lse)
+        torch.cuda.synchronize()
+        assert clove_lib.device_error() == 0
+        for i, m in enumerate(lens):
+            k, v = (ref.rows(c, "bshd", table[i], m, 16) for c in (cache.K, cache.V))
+            o, l, b_o, b_l = _bound(Q[i], k, v, scale, F16)
+            err, tol = (O[i].double() - o).abs(), b_o + ref.half_step(o.abs() + b_o, BF16)
+            assert torch.all(err <= tol), (top, i, float((err / tol).max()))
+            assert torch.all((lse[i].double() - l).abs() <= b_l), (top, i, float(((lse[i].double() - l).abs() / b_l).max()))
