@@ -227,6 +227,8 @@ int clove_qk_norm_rope(const void* Q, const void* K, const void* V, long long q_
     if (cache->num_kv_heads != num_kv_heads || cache->head_dim != head_dim)
       return fail(CLOVE_ERR_INVALID_ARG, "the cache has %d heads of %d, K has %d of %d", cache->num_kv_heads,
                   cache->head_dim, num_kv_heads, head_dim);
+    if (!std::isfinite(1.f / cache->k_scale) || !std::isfinite(1.f / cache->v_scale))
+      return fail(CLOVE_ERR_INVALID_ARG, "cache: a scale's inverse exceeds fp32");
     if (num_tokens > 0 && (V == nullptr || slots == nullptr))
       return fail(CLOVE_ERR_INVALID_ARG, "a cache needs V and slots");
     cache_dtype = cache->dtype;
@@ -286,6 +288,10 @@ int clove_paged_attention(const void* Q, long long q_stride, const clove_paged_c
                 cache->num_kv_heads);
   if (!(scale > 0.f) || !std::isfinite(scale))
     return fail(CLOVE_ERR_INVALID_ARG, "scale must be positive and finite");
+  // Scores are multiplied by this. Subnormal, it would have lost its digits.
+  p.scale_log2 = scale * p.cache.k_scale * 1.4426950408889634f;
+  if (!std::isnormal(p.scale_log2))
+    return fail(CLOVE_ERR_INVALID_ARG, "scale * k_scale leaves the range of fp32");
   if (window < 0) return fail(CLOVE_ERR_INVALID_ARG, "negative window");
   if (max_pages < 0) return fail(CLOVE_ERR_INVALID_ARG, "negative max_pages");
   if (batch == 0) return CLOVE_OK;
@@ -322,7 +328,6 @@ int clove_paged_attention(const void* Q, long long q_stride, const clove_paged_c
   const int hb = D <= 128 && p.group > 8 ? 16 : 8;
   p.blocks = (p.group + hb - 1) / hb;
   p.window = window;
-  p.scale_log2 = scale * p.cache.k_scale * 1.4426950408889634f;
   p.v_scale = p.cache.v_scale;
   p.key_weights = key_weights;
   p.accumulate = accumulate != 0;

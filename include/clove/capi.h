@@ -158,7 +158,9 @@ int clove_flash_attention(const void* Q, const void* K, const void* V, void* O, 
 /* the others any multiple of 16 bytes, e.g. [pages, page_size, heads, D] or    */
 /* [pages, heads, page_size, D]. dtype: the operands' 16-bit type, or e4m3 (8   */
 /* bits; a stored value x stands for x * k_scale or x * v_scale; the scales are */
-/* 1 for 16-bit caches). head_dim 64, 128 or 256.                               */
+/* 1 for 16-bit caches). head_dim 64, 128 or 256. Scales whose inverse (when    */
+/* rows are stored) or whose product with the attention's scale and log2(e)     */
+/* leaves fp32's normal range are refused.                                      */
 /* Index arrays are int32 on the device and are read there: sequences may grow  */
 /* between the replays of a captured call. An index outside its range is never  */
 /* followed; the kernel sets device error 3 (clove_get_device_error).           */

@@ -157,3 +157,22 @@ def test_plain_statements_agree():
     w = [r.choice([0.0, 1.0, 2.0, float("nan")]) for _ in range(40)]
     got = ref.evict(w, 40, 10, 3)
     assert len(got) == 10 and got == sorted(got) and got[-3:] == [37, 38, 39]
+
+
+TINY, HUGE = 1e-39, 3e38
+
+
+@pytest.mark.parametrize("kw,scale", [
+    (dict(dtype=2, k_scale=1e30), 1e30), (dict(dtype=2, k_scale=HUGE), 3.0), (dict(), HUGE),
+    (dict(dtype=2, k_scale=1e-25), 1e-25), (dict(), 1e-45),
+])
+def test_attention_scales_out_of_range(clove_lib, kw, scale):
+    """scale * k_scale * log2(e) must be a finite fp32 number that has not lost its digits:
+    scores would be NaN, or all zero."""
+    assert _attn(clove_lib.lib(), _cache(**kw), scale=scale) == 1
+
+
+@pytest.mark.parametrize("kw", [dict(dtype=2, k_scale=TINY), dict(dtype=2, v_scale=TINY)])
+def test_cache_scales_without_an_inverse(clove_lib, kw):
+    """Scales whose inverse is no fp32 number: rows are stored times the inverse."""
+    assert _rope(clove_lib.lib(), _cache(**kw), V=A, slots=A, vs=256) == 1
