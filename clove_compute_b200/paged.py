@@ -90,6 +90,8 @@ def _gpu(t, name):
 def _elsewhere(fn, index, stream, *args):
     """fn(..., stream handle) for a stream or device other than the current one. The stream
     is current while outputs are allocated, so that their memory belongs to it."""
+    if isinstance(stream, torch.cuda.Stream) and stream.device.index != index:
+        raise ValueError(f"stream must be on GPU {index}, the tensors' own; it is on {stream.device}")
     with torch.cuda.device(index):
         if stream is None:
             return fn(*args, _raw_stream(index))
