@@ -29,8 +29,8 @@ enum Code { kF16, kBF16, kE4M3, kF32, kI32, kCodes };
 static const char* const kNames[kCodes] = {"torch.float16", "torch.bfloat16", "torch.float8_e4m3fn",
                                            "torch.float32", "torch.int32"};
 static PyObject* g_dtype[kCodes];
-static PyObject *g_empty_like, *g_empty_like_kw, *g_contiguous, *g_device, *g_stream, *g_check;
-static PyObject *s_dtype, *s_shape, *s_stride, *s_data_ptr, *s_get_device, *s_new_empty;
+static PyObject *g_empty_like, *g_empty_like_kw, *g_contiguous, *g_device, *g_stream, *g_check, *g_cache;
+static PyObject *s_dtype, *s_shape, *s_stride, *s_data_ptr, *s_get_device, *s_new_empty, *s_key;
 
 #define MAX_DIMS 4
 typedef struct {
@@ -163,17 +163,27 @@ static int fits(long long v, const char* what) {
   return 0;
 }
 
-/* (address, GPU) of a PagedCache. */
-static const clove_paged_cache* cache_of(PyObject* key, int index) {
-  if (!PyTuple_Check(key) || PyTuple_GET_SIZE(key) != 2) {
-    PyErr_SetString(PyExc_TypeError, "cache must be a PagedCache");
+/* What a PagedCache describes; its GPU is *index, or is put there where that is -1. (Its _key
+ * is (address, GPU); no other object's numbers are followed.) */
+static const clove_paged_cache* cache_of(PyObject* cache, int* index) {
+  const int is = PyObject_IsInstance(cache, g_cache);
+  if (is <= 0) {
+    if (is == 0) PyErr_SetString(PyExc_TypeError, "cache must be a PagedCache");
     return NULL;
   }
-  const clove_paged_cache* c = PyLong_AsVoidPtr(PyTuple_GET_ITEM(key, 0));
-  const long at = PyLong_AsLong(PyTuple_GET_ITEM(key, 1));
+  PyObject* key = PyObject_GetAttr(cache, s_key);
+  if (key == NULL) return NULL;
+  const clove_paged_cache* c = NULL;
+  long at = -1;
+  if (PyTuple_Check(key) && PyTuple_GET_SIZE(key) == 2) {
+    c = PyLong_AsVoidPtr(PyTuple_GET_ITEM(key, 0));
+    at = PyLong_AsLong(PyTuple_GET_ITEM(key, 1));
+  }
+  Py_DECREF(key); /* the struct lives as long as the cache */
   if (PyErr_Occurred()) return NULL;
-  if (index >= 0 && at != index) {
-    PyErr_Format(PyExc_ValueError, "the cache must be on GPU %d", index);
+  if (*index < 0) *index = (int)at;
+  if (c == NULL || at != *index) {
+    PyErr_Format(PyExc_ValueError, "the cache must be on GPU %d", *index);
     return NULL;
   }
   return c;
@@ -244,7 +254,8 @@ static PyObject* qk_norm_rope(PyObject* self, PyObject* const* a, Py_ssize_t n) 
   Tensor q, k, t, pos, qw, kw, v, slots, qo, ko;
   qw.ptr = kw.ptr = v.ptr = slots.ptr = qo.ptr = ko.ptr = NULL;
   if (!take(&q, a[0], "Q") || !operand(&q)) return NULL;
-  const int code = q.code, index = q.index;
+  const int code = q.code;
+  int index = q.index;
   void* s = NULL;
   const int here = stream_of(a[13], index, &s);
   if (here == 0) return NULL;
@@ -272,7 +283,7 @@ static PyObject* qk_norm_rope(PyObject* self, PyObject* const* a, Py_ssize_t n) 
       PyErr_SetString(PyExc_ValueError, "a cache needs V and slots");
       return NULL;
     }
-    if (!(cache = cache_of(a[9], index)) || !take(&v, a[8], "V") || !take(&slots, a[10], "slots") ||
+    if (!(cache = cache_of(a[9], &index)) || !take(&v, a[8], "V") || !take(&slots, a[10], "slots") ||
         !heads(&v, code, index, kv, &vs) || !dense1(&slots, kI32, index, T))
       return NULL;
   } else if (GIVEN(a[8]) || GIVEN(a[10])) {
@@ -324,12 +335,13 @@ static PyObject* paged_attention(PyObject* self, PyObject* const* a, Py_ssize_t 
   Tensor q, pt, sl, lse, kw, o;
   lse.ptr = kw.ptr = NULL;
   if (!take(&q, a[0], "Q") || !operand(&q)) return NULL;
-  const int code = q.code, index = q.index;
+  const int code = q.code;
+  int index = q.index;
   void* s = NULL;
   const int here = stream_of(a[10], index, &s);
   if (here == 0) return NULL;
   if (here < 0) Py_RETURN_NOTIMPLEMENTED;
-  const clove_paged_cache* c = cache_of(a[1], index);
+  const clove_paged_cache* c = cache_of(a[1], &index);
   if (c == NULL) return NULL;
   const long long B = q.size[0], H = q.size[1], D = q.size[2];
   if (D != c->head_dim) {
@@ -375,9 +387,9 @@ static PyObject* paged_attention(PyObject* self, PyObject* const* a, Py_ssize_t 
 static PyObject* evict_cache(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   (void)self;
   if (!wants(n, 8)) return NULL;
-  const clove_paged_cache* c = cache_of(a[0], -1);
+  int index = -1;
+  const clove_paged_cache* c = cache_of(a[0], &index);
   if (c == NULL) return NULL;
-  const int index = (int)PyLong_AsLong(PyTuple_GET_ITEM(a[0], 1));
   void* s = NULL;
   const int here = stream_of(a[7], index, &s);
   if (here == 0) return NULL;
@@ -422,12 +434,13 @@ static PyObject* evict_cache(PyObject* self, PyObject* const* a, Py_ssize_t n) {
 }
 
 /* init(library path, (dtypes), empty_like, contiguous_format, current device, current stream,
- *      check) */
+ *      check, PagedCache) */
 static PyObject* init(PyObject* self, PyObject* args) {
   (void)self;
   const char* path;
-  PyObject *dtypes, *like, *format, *device, *stream, *check;
-  if (!PyArg_ParseTuple(args, "sO!OOOOO", &path, &PyTuple_Type, &dtypes, &like, &format, &device, &stream, &check))
+  PyObject *dtypes, *like, *format, *device, *stream, *check, *cache;
+  if (!PyArg_ParseTuple(args, "sO!OOOOOO", &path, &PyTuple_Type, &dtypes, &like, &format, &device, &stream, &check,
+                        &cache))
     return NULL;
   if (PyTuple_GET_SIZE(dtypes) != kCodes) return PyErr_Format(PyExc_ValueError, "%d dtypes expected", kCodes);
   void* lib = dlopen(path, RTLD_NOW | RTLD_LOCAL);
@@ -449,8 +462,11 @@ static PyObject* init(PyObject* self, PyObject* args) {
   s_data_ptr = PyUnicode_InternFromString("data_ptr");
   s_get_device = PyUnicode_InternFromString("get_device");
   s_new_empty = PyUnicode_InternFromString("new_empty");
-  if (!g_empty_like_kw || !s_dtype || !s_shape || !s_stride || !s_data_ptr || !s_get_device || !s_new_empty)
+  s_key = PyUnicode_InternFromString("_key");
+  if (!g_empty_like_kw || !s_dtype || !s_shape || !s_stride || !s_data_ptr || !s_get_device || !s_new_empty ||
+      !s_key)
     return NULL;
+  g_cache = Py_NewRef(cache);
   g_check = Py_NewRef(check);
   Py_RETURN_NONE;
 }

@@ -76,7 +76,7 @@ def _load():
     if _fast is None:
         f = fastcall()
         f.init(library_path(), (torch.float16, torch.bfloat16, torch.float8_e4m3fn, torch.float32, torch.int32),
-               torch.empty_like, torch.contiguous_format, _current_device, _raw_stream, check)
+               torch.empty_like, torch.contiguous_format, _current_device, _raw_stream, check, PagedCache)
         _fast = f
     return _fast
 
@@ -122,13 +122,12 @@ def qk_norm_rope(Q, K, rope_table, positions, q_weight=None, k_weight=None, eps:
     K_out K. Negative positions mark padding tokens (nothing written), negative slots
     tokens that are not stored; other slots must differ."""
     fn = (_fast or _load()).qk_norm_rope
-    key = getattr(cache, "_key", cache)
     if stream is None:
-        r = fn(Q, K, rope_table, positions, q_weight, k_weight, eps, interleaved, V, key, slots, Q_out, K_out, None)
+        r = fn(Q, K, rope_table, positions, q_weight, k_weight, eps, interleaved, V, cache, slots, Q_out, K_out, None)
         if r is not NotImplemented:
             return r
     return _elsewhere(fn, _gpu(Q, "Q"), stream, Q, K, rope_table, positions, q_weight, k_weight, eps, interleaved,
-                      V, key, slots, Q_out, K_out)
+                      V, cache, slots, Q_out, K_out)
 
 
 def paged_attention(Q, cache: PagedCache, page_table, seq_lens, scale: float | None = None,
@@ -143,12 +142,11 @@ def paged_attention(Q, cache: PagedCache, page_table, seq_lens, scale: float | N
     key, summed over its query heads (added with accumulate=True); no page may then be in
     two sequences. scale defaults to 1/sqrt(D). An empty sequence gives zeros and -inf."""
     fn = (_fast or _load()).paged_attention
-    key = getattr(cache, "_key", cache)
     if stream is None:
-        r = fn(Q, key, page_table, seq_lens, scale, window, lse, key_weights, accumulate, O, None)
+        r = fn(Q, cache, page_table, seq_lens, scale, window, lse, key_weights, accumulate, O, None)
         if r is not NotImplemented:
             return r
-    return _elsewhere(fn, _gpu(Q, "Q"), stream, Q, key, page_table, seq_lens, scale, window, lse,
+    return _elsewhere(fn, _gpu(Q, "Q"), stream, Q, cache, page_table, seq_lens, scale, window, lse,
                       key_weights, accumulate, O)
 
 
@@ -163,8 +161,8 @@ def evict_cache(cache: PagedCache, key_weights, page_table, seq_lens, dst_table,
     if not isinstance(cache, PagedCache):
         raise TypeError("cache must be a PagedCache")
     if stream is None:
-        r = fn(cache._key, key_weights, page_table, seq_lens, dst_table, budget, recent, None)
+        r = fn(cache, key_weights, page_table, seq_lens, dst_table, budget, recent, None)
         if r is not NotImplemented:
             return r
-    return _elsewhere(fn, cache.index, stream, cache._key, key_weights, page_table, seq_lens, dst_table, budget,
+    return _elsewhere(fn, cache.index, stream, cache, key_weights, page_table, seq_lens, dst_table, budget,
                       recent)
