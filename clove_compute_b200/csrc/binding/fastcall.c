@@ -79,6 +79,8 @@ static int take(Tensor* t, PyObject* o, const char* name) {
   Py_XDECREF(dev);
   Py_XDECREF(ptr);
   if (!ok) {
+    /* A tensor without storage, in torch's own words. */
+    if (PyErr_Occurred() && PyErr_ExceptionMatches(PyExc_RuntimeError)) return 0;
     PyErr_Clear();
     PyErr_Format(PyExc_TypeError, "%s must be a torch.Tensor", name);
   }

@@ -52,3 +52,15 @@ def test_only_a_paged_cache_is_followed():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", _NOT_A_CACHE], cwd=root, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and r.stdout.strip() == "refused", (r.returncode, r.stdout, r.stderr[-1500:])
+
+
+def test_torchs_own_refusals_are_passed_on():
+    """A tensor without storage (under vmap, a transform or tracing) is refused with torch's
+    reason, what is no tensor as such."""
+    q = torch.zeros(2, 3, 4, 128, dtype=torch.float16)
+    for call in (lambda x: cc.paged_attention(x, None, None, None), lambda x: cc.qk_norm_rope(x, x, None, None)):
+        with pytest.raises(RuntimeError, match="storage"):
+            torch.vmap(call)(q)
+        for wrong in ("text", None, 3, [1.0]):
+            with pytest.raises(TypeError, match="Q must be a torch.Tensor"):
+                call(wrong)
