@@ -5,7 +5,7 @@ arch=compute_100a,code=sm_100a``); nvcc cross-compiles without a GPU. Objects
 go to ``clove_compute_b200/_build/`` and are rebuilt when a source or any
 header under ``csrc/`` or ``include/`` is newer. Run ``python -m
 clove_compute_b200.build`` (``-v`` prints ptxas register / spill reports). The CPython
-entry points (``csrc/binding/fastcall.c``) become ``_fastcall.so`` beside it; without
+entry points (``csrc/binding/fastcall.c``) become ``_fastcall.<tag>.so`` beside it; without
 Python's headers they are left out, and the paged-cache functions raise ImportError.
 """
 from __future__ import annotations
@@ -23,7 +23,8 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libclove_b200.so")
-FASTCALL = os.path.join(PKG, "_fastcall.so")
+# (Tagged, e.g. _fastcall.cpython-312-x86_64-linux-gnu.so: it belongs to one Python version.)
+FASTCALL = os.path.join(PKG, "_fastcall" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = [
@@ -67,6 +68,9 @@ def _compile(src: str, verbose: bool) -> str:
 
 def _build_fastcall(force: bool) -> None:
     src = os.path.join(CSRC, "binding", "fastcall.c")
+    untagged = os.path.join(os.path.dirname(FASTCALL), "_fastcall.so")  # any version would load it
+    if untagged != FASTCALL and os.path.exists(untagged):
+        os.remove(untagged)
     newest = max(os.path.getmtime(src), os.path.getmtime(os.path.join(ROOT, "include", "clove", "capi.h")))
     if not force and os.path.exists(FASTCALL) and os.path.getmtime(FASTCALL) >= newest:
         return
