@@ -52,12 +52,13 @@ int scratch_alloc(void** out, size_t bytes, int device, bool capturing, cudaStre
 // results. Calls that can overlap on the GPU must not share one:
 // * each stream keeps its own (by the stream's id: a destroyed stream's handle may return
 //   as another stream's, and every thread's default stream has the same handle);
-// * each captured call gets counters that no other call ever gets, and partial results from
-//   the graph's memory, since its graph may be replayed beside anything.
-// Counters come from an array in the library, 1 MB per device (over 800 calls and streams);
-// when it is used up, or its address is not known yet under capture, a call brings its own
-// and clears them first.
-constexpr int kMaxCtas = 1024;
+// * a captured call's graph may be replayed beside anything: it gets partial results from the
+//   graph's memory and counters that no call outside its graph ever gets. Calls of one graph
+//   share them where the graph itself orders them (find_counters). (Its memory also keeps a
+//   graph from having two instances at a time.)
+// Counters come from an array in the library, 1 MB per device: two per SM for each stream
+// and each chain of captured calls, enough for about 800. When it is used up, or its address
+// is not known yet under capture, a call brings its own and clears them first.
 constexpr size_t kKeptParts = 8u << 20;
 constexpr int kMaxKept = 64;
 struct KeptWorkspace {
@@ -65,11 +66,21 @@ struct KeptWorkspace {
   unsigned* counters;
   float* parts;
 };
+// Counters of captured calls, and the node that ends the last call that took them (null: one
+// is being captured). The latest kMaxCaptures are found again.
+constexpr int kMaxCaptures = 64;
+struct CaptureCounters {
+  unsigned long long capture_id;
+  cudaGraphNode_t last;
+  unsigned* counters;
+};
 struct DeviceWorkspaces {
   unsigned* base = nullptr;  // the device's counters
   int used = 0;
   int kept_count = 0;
   KeptWorkspace kept[kMaxKept];
+  CaptureCounters captures[kMaxCaptures] = {};
+  unsigned next_capture = 0;
 };
 std::mutex g_ws_mu;
 DeviceWorkspaces g_ws[64];
@@ -79,6 +90,7 @@ struct Workspace {
   float* parts = nullptr;
   void* own = nullptr;  // to be released after the call
   bool capturing = false;
+  unsigned long long capture_id = 0;
 };
 
 // `count` counters that nobody else has, or null.
@@ -89,23 +101,62 @@ unsigned* reserve_counters(DeviceWorkspaces& d, int count) {
   return c;
 }
 
-int take_workspace(Workspace* w, int ctas, size_t part_bytes, int device, cudaStream_t s) {
+// Counters of an earlier call of this capture that is over, in every replay, before the work
+// that is captured on `s` next: one whose last node is reached from the stream's
+// dependencies. (The last node frees the partial results and so follows the kernels in full;
+// what starts after it, programmatically overlapped or not, starts after them.) The search
+// ends after kMaxVisited nodes: a model's layer has a few dozen between two calls.
+constexpr int kMaxVisited = 512, kMaxEdges = 16;
+unsigned* find_counters(DeviceWorkspaces& d, unsigned long long capture_id, const cudaGraphNode_t* deps, size_t n) {
+  cudaGraphNode_t seen[kMaxVisited];
+  int count = 0;
+  auto visit = [&](cudaGraphNode_t node) {
+    for (int i = 0; i < count; ++i)
+      if (seen[i] == node) return;
+    if (count < kMaxVisited) seen[count++] = node;
+  };
+  for (size_t i = 0; i < n; ++i) visit(deps[i]);
+  for (int at = 0; at < count; ++at) {
+    for (CaptureCounters& c : d.captures)
+      if (c.capture_id == capture_id && c.last == seen[at]) {
+        c.last = nullptr;
+        return c.counters;
+      }
+    cudaGraphNode_t before[kMaxEdges];
+    cudaGraphEdgeData edges[kMaxEdges];
+    size_t m = kMaxEdges;
+    if (cudaGraphNodeGetDependencies_v2(seen[at], before, edges, &m) != cudaSuccess) return nullptr;
+    for (size_t i = 0; i < m && i < kMaxEdges; ++i)
+      if (before[i] != nullptr) visit(before[i]);
+  }
+  return nullptr;
+}
+
+// (ctas is at most the device's `most`, two per SM.)
+int take_workspace(Workspace* w, int ctas, size_t part_bytes, const DeviceInfo& dev, cudaStream_t s) {
+  const int device = dev.device, most = (2 * dev.num_sms + 31) & ~31;
   cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-  int rc = check_cuda(cudaStreamIsCapturing(s, &cap), "cudaStreamIsCapturing");
+  unsigned long long id = 0;
+  const cudaGraphNode_t* deps = nullptr;
+  const cudaGraphEdgeData* edges = nullptr;
+  size_t num_deps = 0;
+  int rc = check_cuda(cudaStreamGetCaptureInfo_v3(s, &cap, &w->capture_id, nullptr, &deps, &edges, &num_deps),
+                      "cudaStreamGetCaptureInfo");
   if (rc) return rc;
   w->capturing = cap != cudaStreamCaptureStatusNone;
-  if (ctas > kMaxCtas || part_bytes > kKeptParts)
-    return fail(CLOVE_ERR_UNSUPPORTED, "paged_attention: workspace of %d CTAs", ctas);
-  unsigned long long id = 0;
-  if (!w->capturing) {
+  if (!w->capturing) {  // (the id of a capturing stream cannot be asked for)
     rc = check_cuda(cudaStreamGetId(s, &id), "cudaStreamGetId");
     if (rc) return rc;
   }
+  if (ctas > most || part_bytes > kKeptParts)
+    return fail(CLOVE_ERR_UNSUPPORTED, "paged_attention: workspace of %d CTAs", ctas);
   {
     std::lock_guard<std::mutex> lock(g_ws_mu);
     DeviceWorkspaces& d = g_ws[device & 63];
     if (w->capturing) {
-      w->counters = reserve_counters(d, (ctas + 31) & ~31);
+      w->counters = find_counters(d, w->capture_id, deps, num_deps);
+      if (w->counters == nullptr && (w->counters = reserve_counters(d, most)) != nullptr)
+        d.captures[d.next_capture++ % kMaxCaptures] = CaptureCounters{w->capture_id, nullptr, w->counters};
     } else {
       for (int i = 0; i < d.kept_count; ++i)
         if (d.kept[i].stream_id == id) {
@@ -118,7 +169,7 @@ int take_workspace(Workspace* w, int ctas, size_t part_bytes, int device, cudaSt
         if (rc) return rc;
       }
       if (d.kept_count < kMaxKept) {
-        unsigned* c = reserve_counters(d, kMaxCtas);
+        unsigned* c = reserve_counters(d, most);
         if (c != nullptr) {
           void* parts = nullptr;
           rc = scratch_alloc(&parts, kKeptParts, device, false, s);
@@ -132,7 +183,7 @@ int take_workspace(Workspace* w, int ctas, size_t part_bytes, int device, cudaSt
     }
   }
   // Partial results, and counters where none were left, for this call alone.
-  const size_t head = w->counters == nullptr ? kMaxCtas * sizeof(unsigned) : 0;
+  const size_t head = w->counters == nullptr ? static_cast<size_t>(most) * sizeof(unsigned) : 0;
   rc = scratch_alloc(&w->own, head + part_bytes, device, w->capturing, s);
   if (rc) return rc;
   w->parts = reinterpret_cast<float*>(static_cast<char*>(w->own) + head);
@@ -144,9 +195,23 @@ int take_workspace(Workspace* w, int ctas, size_t part_bytes, int device, cudaSt
   return rc;
 }
 
-int drop_workspace(Workspace* w, cudaStream_t s) {
+int drop_workspace(Workspace* w, int device, cudaStream_t s) {
   if (w->own == nullptr) return CLOVE_OK;
-  return check_cuda(cudaFreeAsync(w->own, s), "cudaFreeAsync(paged attention)");
+  const int rc = check_cuda(cudaFreeAsync(w->own, s), "cudaFreeAsync(paged attention)");
+  if (rc || !w->capturing) return rc;
+  // The node that a later call has to follow to take the same counters.
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  const cudaGraphNode_t* deps = nullptr;
+  const cudaGraphEdgeData* edges = nullptr;
+  size_t num_deps = 0;
+  if (cudaStreamGetCaptureInfo_v3(s, &cap, &id, nullptr, &deps, &edges, &num_deps) != cudaSuccess ||
+      id != w->capture_id || num_deps != 1)
+    return CLOVE_OK;
+  std::lock_guard<std::mutex> lock(g_ws_mu);
+  for (CaptureCounters& c : g_ws[device & 63].captures)
+    if (c.capture_id == id && c.counters == w->counters) c.last = deps[0];
+  return CLOVE_OK;
 }
 
 // Checks a cache description and converts it; `dtype` is the 16-bit type it is used with.
@@ -341,7 +406,7 @@ int clove_paged_attention(const void* Q, long long q_stride, const clove_paged_c
   const size_t scores = static_cast<size_t>(batch) * num_heads * static_cast<size_t>(capacity) * 4;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   Workspace ws;
-  rc = take_workspace(&ws, ctas, static_cast<size_t>(ctas) * 2 * hb * (D + 2) * 4, dev.device, s);
+  rc = take_workspace(&ws, ctas, static_cast<size_t>(ctas) * 2 * hb * (D + 2) * 4, dev, s);
   if (rc) return rc;
   p.counters = ws.counters;
   p.part_o = ws.parts;
@@ -362,7 +427,7 @@ int clove_paged_attention(const void* Q, long long q_stride, const clove_paged_c
     const int rc2 = check_cuda(cudaFreeAsync(sc, s), "cudaFreeAsync(paged attention scores)");
     if (!rc) rc = rc2;
   }
-  const int rc2 = drop_workspace(&ws, s);
+  const int rc2 = drop_workspace(&ws, dev.device, s);
   return rc ? rc : rc2;
 }
 

@@ -1,0 +1,110 @@
+"""What paged attention keeps between calls: counters and partial results, per stream and
+per graph (each test in a process of its own: both are the process's)."""
+import os
+import subprocess
+import sys
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+_SETUP = r"""
+import torch
+import clove_compute_b200 as cc
+from cuda.bindings import runtime as rt
+g = torch.Generator(device="cuda").manual_seed(1)
+K, V = (torch.randn((400, 16, 2, 128), device="cuda", generator=g).half() for _ in range(2))
+c = cc.PagedCache(K, V)
+table = torch.randperm(400, device="cuda", generator=g)[:380].to(torch.int32).view(2, 190)
+sl = torch.tensor([3000, 77], dtype=torch.int32, device="cuda")
+Q = torch.randn((2, 8, 128), device="cuda", generator=g).half()
+def ok(r):
+    assert int(r[0]) == 0, r
+    return r[1] if len(r) == 2 else r[1:]
+"""
+
+
+def _run(code, done):
+    r = subprocess.run([sys.executable, "-c", _SETUP + code], cwd=ROOT, capture_output=True, text=True, timeout=600)
+    assert r.returncode == 0 and done in r.stdout, (r.stdout[-500:], r.stderr[-2500:])
+
+
+_MANY_CAPTURES = r"""
+want = cc.paged_attention(Q, c, table, sl)
+torch.cuda.synchronize()
+memsets = []
+graphs = []
+for k in range(20):
+    gr = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(gr):
+        outs = [cc.paged_attention(Q, c, table, sl) for _ in range(80)]
+    gr.instantiate()
+    raw = rt.cudaGraph_t(gr.raw_cuda_graph())
+    _, n = ok(rt.cudaGraphGetNodes(raw, 0))
+    nodes, _ = ok(rt.cudaGraphGetNodes(raw, n))
+    memsets.append(sum(ok(rt.cudaGraphNodeGetType(x)) == rt.cudaGraphNodeType.cudaGraphNodeTypeMemset for x in nodes))
+    graphs.append((gr, outs))
+for _ in range(2):
+    for gr, outs in graphs:
+        for o in outs:
+            o.zero_()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for (gr, outs), s in zip(graphs, streams):
+        with torch.cuda.stream(s):
+            gr.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for _, outs in graphs for o in outs)
+assert cc.device_error() == 0
+print("memsets", memsets)
+assert sum(memsets) == 0, memsets
+print("captures ok")
+"""
+
+
+def test_captured_models_share_counters_in_their_graph(cuda):
+    """Twenty graphs of eighty calls, as of a model captured at twenty batch sizes: none
+    needs counters of its own to be cleared, and their replays, side by side too, are right."""
+    _run(_MANY_CAPTURES, "captures ok")
+
+
+_FORKED = r"""
+lens = [torch.tensor([3000 - 700 * i, 77 + i], dtype=torch.int32, device="cuda") for i in range(4)]
+want = [cc.paged_attention(Q, c, table, n) for n in lens]
+torch.cuda.synchronize()
+gr = torch.cuda.CUDAGraph()
+side = [torch.cuda.Stream() for _ in range(3)]
+with torch.cuda.graph(gr):
+    main = torch.cuda.current_stream()
+    fork = torch.cuda.Event()
+    fork.record(main)
+    outs = []
+    for rep in range(5):
+        outs.append((0, cc.paged_attention(Q, c, table, lens[0])))
+        for i, s in enumerate(side):
+            s.wait_event(fork)
+            outs.append((i + 1, cc.paged_attention(Q, c, table, lens[i + 1], stream=s)))
+    for again in range(3):  # main goes on after the others, they beside it
+        for s in side:
+            join = torch.cuda.Event()
+            join.record(s)
+            main.wait_event(join)
+        if again < 2:
+            outs.append((0, cc.paged_attention(Q, c, table, lens[0])))
+            for i, s in enumerate(side):
+                outs.append((i + 1, cc.paged_attention(Q, c, table, lens[i + 1], stream=s)))
+for _ in range(20):
+    for _, o in outs:
+        o.zero_()
+    gr.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i]) for i, o in outs)
+assert cc.device_error() == 0
+print("forked ok")
+"""
+
+
+def test_streams_forked_in_one_capture(cuda):
+    """Calls on four streams of one capture run beside each other when it is replayed."""
+    _run(_FORKED, "forked ok")
