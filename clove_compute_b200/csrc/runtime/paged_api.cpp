@@ -17,6 +17,16 @@ namespace {
 
 inline bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
+// While it lives, this thread's allocations outside a capture neither fail because another
+// thread captures (in the default, global mode) nor spoil its capture.
+struct OutsideCaptures {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  OutsideCaptures() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~OutsideCaptures() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  OutsideCaptures(const OutsideCaptures&) = delete;
+  OutsideCaptures& operator=(const OutsideCaptures&) = delete;
+};
+
 // Stream-ordered scratch that stays with the process between calls, one pool per device;
 // under stream capture an allocation of the graph's own.
 std::mutex g_pool_mu;
@@ -24,6 +34,7 @@ cudaMemPool_t g_pool[64];
 
 int scratch_alloc(void** out, size_t bytes, int device, bool capturing, cudaStream_t s) {
   if (capturing) return check_cuda(cudaMallocAsync(out, bytes, s), "cudaMallocAsync(paged attention)");
+  const OutsideCaptures outside;
   cudaMemPool_t pool;
   {
     std::lock_guard<std::mutex> lock(g_pool_mu);
@@ -46,6 +57,12 @@ int scratch_alloc(void** out, size_t bytes, int device, bool capturing, cudaStre
     pool = g_pool[device & 63];
   }
   return check_cuda(cudaMallocFromPoolAsync(out, bytes, pool, s), "cudaMallocFromPoolAsync(paged attention)");
+}
+
+int scratch_free(void* p, bool capturing, cudaStream_t s) {
+  if (capturing) return check_cuda(cudaFreeAsync(p, s), "cudaFreeAsync(paged attention)");
+  const OutsideCaptures outside;
+  return check_cuda(cudaFreeAsync(p, s), "cudaFreeAsync(paged attention)");
 }
 
 // Workspace of the attention kernel: per-CTA counters, zero between calls, and partial
@@ -165,6 +182,7 @@ int take_workspace(Workspace* w, int ctas, size_t part_bytes, const DeviceInfo& 
           return CLOVE_OK;
         }
       if (d.base == nullptr) {
+        const OutsideCaptures outside;
         rc = paged_counter_base(&d.base);
         if (rc) return rc;
       }
@@ -190,14 +208,14 @@ int take_workspace(Workspace* w, int ctas, size_t part_bytes, const DeviceInfo& 
   if (head != 0) {
     w->counters = static_cast<unsigned*>(w->own);
     rc = check_cuda(cudaMemsetAsync(w->own, 0, head, s), "cudaMemsetAsync(paged attention)");
-    if (rc) cudaFreeAsync(w->own, s);
+    if (rc) scratch_free(w->own, w->capturing, s);
   }
   return rc;
 }
 
 int drop_workspace(Workspace* w, int device, cudaStream_t s) {
   if (w->own == nullptr) return CLOVE_OK;
-  const int rc = check_cuda(cudaFreeAsync(w->own, s), "cudaFreeAsync(paged attention)");
+  const int rc = scratch_free(w->own, w->capturing, s);
   if (rc || !w->capturing) return rc;
   // The node that a later call has to follow to take the same counters.
   cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
@@ -424,7 +442,7 @@ int clove_paged_attention(const void* Q, long long q_stride, const clove_paged_c
     rc = dtype == CLOVE_DTYPE_F16 ? launch_paged_attention_f16(p, D, hb, e4m3, ctas, dev, s)
                                   : launch_paged_attention_bf16(p, D, hb, e4m3, ctas, dev, s);
   if (sc != nullptr) {
-    const int rc2 = check_cuda(cudaFreeAsync(sc, s), "cudaFreeAsync(paged attention scores)");
+    const int rc2 = scratch_free(sc, ws.capturing, s);
     if (!rc) rc = rc2;
   }
   const int rc2 = drop_workspace(&ws, dev.device, s);

@@ -108,3 +108,50 @@ print("forked ok")
 def test_streams_forked_in_one_capture(cuda):
     """Calls on four streams of one capture run beside each other when it is replayed."""
     _run(_FORKED, "forked ok")
+
+
+_CAPTURE_BESIDE_EAGER = r"""
+import sys, threading
+cold = sys.argv[1] == "cold"
+O = torch.empty_like(Q)
+w = torch.zeros((400, 2, 16), device="cuda")
+mine, theirs = torch.cuda.Stream(), torch.cuda.Stream()
+want = None
+if not cold:
+    want = cc.paged_attention(Q, c, table, sl)
+x = torch.zeros(1 << 20, device="cuda")
+torch.cuda.synchronize()
+bad = []
+def eager():
+    try:
+        torch.cuda.set_device(0)
+        for s in (theirs, theirs):
+            cc.paged_attention(Q, c, table, sl, O=O, stream=s.cuda_stream)
+            cc.paged_attention(Q, c, table, sl, O=O, key_weights=w, stream=s.cuda_stream)
+    except Exception as e:
+        bad.append(e)
+gr = torch.cuda.CUDAGraph()
+with torch.cuda.graph(gr, stream=mine):
+    x.add_(1)
+    t = threading.Thread(target=eager)
+    t.start()
+    t.join()
+    y = cc.paged_attention(Q, c, table, sl)
+torch.cuda.synchronize()
+assert not bad, bad
+gr.replay()
+torch.cuda.synchronize()
+want = cc.paged_attention(Q, c, table, sl) if want is None else want
+assert torch.equal(y, want) and torch.equal(O, want)
+assert cc.device_error() == 0
+print("beside ok")
+"""
+
+
+@pytest.mark.parametrize("start", ["cold", "warm"])
+def test_eager_calls_while_another_thread_captures(cuda, start):
+    """The eager calls of one thread, the process's first ones too, and a capture under way in
+    another do not disturb each other."""
+    r = subprocess.run([sys.executable, "-c", _SETUP + _CAPTURE_BESIDE_EAGER, start], cwd=ROOT, capture_output=True,
+                       text=True, timeout=600)
+    assert r.returncode == 0 and "beside ok" in r.stdout, (r.stdout[-500:], r.stderr[-2500:])
