@@ -68,7 +68,10 @@ int scratch_free(void* p, bool capturing, cudaStream_t s) {
 // Workspace of the attention kernel: per-CTA counters, zero between calls, and partial
 // results. Calls that can overlap on the GPU must not share one:
 // * each stream keeps its own (by the stream's id: a destroyed stream's handle may return
-//   as another stream's, and every thread's default stream has the same handle);
+//   as another stream's, and every thread's default stream has the same handle). There are
+//   kMaxKept of them; a further stream takes over the least recently used one if that one's
+//   last call is over (its event says so; nothing waits for another stream), or brings one
+//   for the call alone;
 // * a captured call's graph may be replayed beside anything: it gets partial results from the
 //   graph's memory and counters that no call outside its graph ever gets. Calls of one graph
 //   share them where the graph itself orders them (find_counters). (Its memory also keeps a
@@ -77,11 +80,15 @@ int scratch_free(void* p, bool capturing, cudaStream_t s) {
 // and each chain of captured calls, enough for about 800. When it is used up, or its address
 // is not known yet under capture, a call brings its own and clears them first.
 constexpr size_t kKeptParts = 8u << 20;
-constexpr int kMaxKept = 64;
+constexpr int kMaxKept = 16;
 struct KeptWorkspace {
-  unsigned long long stream_id;
-  unsigned* counters;
-  float* parts;
+  unsigned long long stream_id = 0;
+  unsigned* counters = nullptr;
+  float* parts = nullptr;
+  cudaEvent_t event = nullptr;
+  bool recorded = false;        // the event stands behind the latest call
+  int users = 0;                // calls between take_workspace and drop_workspace
+  unsigned long long used = 0;  // when, in calls
 };
 // Counters of captured calls, and the node that ends the last call that took them (null: one
 // is being captured). The latest kMaxCaptures are found again.
@@ -95,6 +102,7 @@ struct DeviceWorkspaces {
   unsigned* base = nullptr;  // the device's counters
   int used = 0;
   int kept_count = 0;
+  unsigned long long calls = 0;
   KeptWorkspace kept[kMaxKept];
   CaptureCounters captures[kMaxCaptures] = {};
   unsigned next_capture = 0;
@@ -108,6 +116,7 @@ struct Workspace {
   void* own = nullptr;  // to be released after the call
   bool capturing = false;
   unsigned long long capture_id = 0;
+  KeptWorkspace* kept = nullptr;  // the stream's
 };
 
 // `count` counters that nobody else has, or null.
@@ -149,6 +158,44 @@ unsigned* find_counters(DeviceWorkspaces& d, unsigned long long capture_id, cons
   return nullptr;
 }
 
+// A workspace for a stream that has none: null where all are in use.
+int new_workspace(DeviceWorkspaces& d, unsigned long long id, int counters, int device, cudaStream_t s,
+                  KeptWorkspace** out) {
+  const OutsideCaptures outside;
+  if (d.base == nullptr) {
+    const int rc = paged_counter_base(&d.base);
+    if (rc) return rc;
+  }
+  if (d.kept_count < kMaxKept) {
+    KeptWorkspace& k = d.kept[d.kept_count];
+    if (k.event == nullptr) {
+      const int rc = check_cuda(cudaEventCreateWithFlags(&k.event, cudaEventDisableTiming), "cudaEventCreate");
+      if (rc) return rc;
+    }
+    if (k.counters == nullptr) k.counters = reserve_counters(d, counters);
+    if (k.counters == nullptr) return CLOVE_OK;
+    void* parts = nullptr;
+    const int rc = scratch_alloc(&parts, kKeptParts, device, false, s);
+    if (rc) return rc;
+    k.parts = static_cast<float*>(parts);
+    k.stream_id = id;
+    ++d.kept_count;
+    *out = &k;
+    return CLOVE_OK;
+  }
+  KeptWorkspace* oldest = nullptr;
+  for (KeptWorkspace& k : d.kept)
+    if (k.users == 0 && k.recorded && (oldest == nullptr || k.used < oldest->used)) oldest = &k;
+  if (oldest == nullptr) return CLOVE_OK;
+  if (cudaEventQuery(oldest->event) != cudaSuccess) {
+    (void)cudaGetLastError();  // (not ready is no error)
+    return CLOVE_OK;
+  }
+  oldest->stream_id = id;
+  *out = oldest;
+  return CLOVE_OK;
+}
+
 // (ctas is at most the device's `most`, two per SM.)
 int take_workspace(Workspace* w, int ctas, size_t part_bytes, const DeviceInfo& dev, cudaStream_t s) {
   const int device = dev.device, most = (2 * dev.num_sms + 31) & ~31;
@@ -175,28 +222,20 @@ int take_workspace(Workspace* w, int ctas, size_t part_bytes, const DeviceInfo& 
       if (w->counters == nullptr && (w->counters = reserve_counters(d, most)) != nullptr)
         d.captures[d.next_capture++ % kMaxCaptures] = CaptureCounters{w->capture_id, nullptr, w->counters};
     } else {
-      for (int i = 0; i < d.kept_count; ++i)
-        if (d.kept[i].stream_id == id) {
-          w->counters = d.kept[i].counters;
-          w->parts = d.kept[i].parts;
-          return CLOVE_OK;
-        }
-      if (d.base == nullptr) {
-        const OutsideCaptures outside;
-        rc = paged_counter_base(&d.base);
+      KeptWorkspace* k = nullptr;
+      for (int i = 0; i < d.kept_count && k == nullptr; ++i)
+        if (d.kept[i].stream_id == id) k = &d.kept[i];
+      if (k == nullptr) {
+        rc = new_workspace(d, id, most, device, s, &k);
         if (rc) return rc;
       }
-      if (d.kept_count < kMaxKept) {
-        unsigned* c = reserve_counters(d, most);
-        if (c != nullptr) {
-          void* parts = nullptr;
-          rc = scratch_alloc(&parts, kKeptParts, device, false, s);
-          if (rc) return rc;
-          d.kept[d.kept_count++] = KeptWorkspace{id, c, static_cast<float*>(parts)};
-          w->counters = c;
-          w->parts = static_cast<float*>(parts);
-          return CLOVE_OK;
-        }
+      if (k != nullptr) {
+        ++k->users;
+        k->used = ++d.calls;
+        w->kept = k;
+        w->counters = k->counters;
+        w->parts = k->parts;
+        return CLOVE_OK;
       }
     }
   }
@@ -214,6 +253,17 @@ int take_workspace(Workspace* w, int ctas, size_t part_bytes, const DeviceInfo& 
 }
 
 int drop_workspace(Workspace* w, int device, cudaStream_t s) {
+  if (w->kept != nullptr) {
+    std::lock_guard<std::mutex> lock(g_ws_mu);
+    KeptWorkspace& k = *w->kept;
+    --k.users;
+    // (One stream alone, as a rule, needs no event: nobody takes over from it.)
+    k.recorded = false;
+    if (g_ws[device & 63].kept_count == 1) return CLOVE_OK;
+    const int rc = check_cuda(cudaEventRecord(k.event, s), "cudaEventRecord(paged attention)");
+    k.recorded = rc == CLOVE_OK;
+    return rc;
+  }
   if (w->own == nullptr) return CLOVE_OK;
   const int rc = scratch_free(w->own, w->capturing, s);
   if (rc || !w->capturing) return rc;

@@ -219,8 +219,9 @@ int clove_qk_norm_rope(const void* Q, const void* K, const void* V, long long q_
  * softmax weight, summed over its query heads, is written there, or added when accumulate
  * != 0; no other entry is touched. No page may then appear in two sequences. It takes
  * batch * num_heads * max_pages * page_size * 4 bytes of scratch.
- * The library keeps 8 MB of workspace for every stream that has made a call, and the
- * scratch of key_weights in a stream-ordered pool; captured calls use the graph's memory.
+ * The library keeps 8 MB of workspace for each of up to 16 streams that have made a call
+ * (further ones take over what is idle, or bring their own for the call), and the scratch
+ * of key_weights in a stream-ordered pool; captured calls use the graph's memory.
  * Calls on different streams, replays of different graphs and calls of different threads
  * may overlap. */
 int clove_paged_attention(const void* Q, long long q_stride, const clove_paged_cache* cache,

@@ -155,3 +155,44 @@ def test_eager_calls_while_another_thread_captures(cuda, start):
     r = subprocess.run([sys.executable, "-c", _SETUP + _CAPTURE_BESIDE_EAGER, start], cwd=ROOT, capture_output=True,
                        text=True, timeout=600)
     assert r.returncode == 0 and "beside ok" in r.stdout, (r.stdout[-500:], r.stderr[-2500:])
+
+
+_STREAMS = r"""
+want = cc.paged_attention(Q, c, table, sl)
+O = torch.empty_like(Q)
+torch.cuda.synchronize()
+free0 = torch.cuda.mem_get_info()[0]
+for rep in range(3):
+    for k in range(100):
+        s = ok(rt.cudaStreamCreate())
+        for _ in range(2):
+            O.zero_()
+            torch.cuda.synchronize()
+            cc.paged_attention(Q, c, table, sl, O=O, stream=int(s))
+        ok(rt.cudaStreamSynchronize(s))
+        assert torch.equal(O, want)
+        ok(rt.cudaStreamDestroy(s))
+torch.cuda.synchronize()
+held = free0 - torch.cuda.mem_get_info()[0]
+print("held", held >> 20, "MB")
+assert held <= 160 << 20, held
+outs = [torch.empty_like(Q) for _ in range(40)]
+streams = [ok(rt.cudaStreamCreate()) for _ in outs]
+for rep in range(20):  # more at a time than workspaces are kept
+    for o in outs:
+        o.zero_()
+    torch.cuda.synchronize()
+    for _ in range(2):
+        for o, s in zip(outs, streams):
+            cc.paged_attention(Q, c, table, sl, O=o, stream=int(s))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+assert cc.device_error() == 0
+print("streams ok")
+"""
+
+
+def test_workspaces_of_gone_streams_are_taken_over(cuda):
+    """Hundreds of streams, one after the other: what is kept stays bounded (16 workspaces of
+    8 MB, and the pool's granularity), and results right; so with 40 in use at once."""
+    _run(_STREAMS, "streams ok")
