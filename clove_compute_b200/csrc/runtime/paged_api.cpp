@@ -27,8 +27,10 @@ struct OutsideCaptures {
   OutsideCaptures& operator=(const OutsideCaptures&) = delete;
 };
 
-// Stream-ordered scratch that stays with the process between calls, one pool per device;
-// under stream capture an allocation of the graph's own.
+// Stream-ordered scratch, one pool per device; under stream capture an allocation of the
+// graph's own. Between calls the pool holds kPoolHolds, the kept workspaces among them; what
+// is above goes back to the device when the program next waits for it.
+constexpr uint64_t kPoolHolds = 512u << 20;
 std::mutex g_pool_mu;
 cudaMemPool_t g_pool[64];
 
@@ -45,7 +47,7 @@ int scratch_alloc(void** out, size_t bytes, int device, bool capturing, cudaStre
       props.location.id = device;
       int rc = check_cuda(cudaMemPoolCreate(&pool, &props), "cudaMemPoolCreate(paged attention)");
       if (rc) return rc;
-      uint64_t keep = UINT64_MAX;
+      uint64_t keep = kPoolHolds;
       rc = check_cuda(cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep),
                       "cudaMemPoolSetAttribute(paged attention)");
       if (rc) {

@@ -218,10 +218,12 @@ int clove_qk_norm_rope(const void* Q, const void* K, const void* V, long long q_
  * key_weights (may be NULL) [num_pages, num_kv_heads, page_size] fp32: each attended key's
  * softmax weight, summed over its query heads, is written there, or added when accumulate
  * != 0; no other entry is touched. No page may then appear in two sequences. It takes
- * batch * num_heads * max_pages * page_size * 4 bytes of scratch.
+ * batch * num_heads * max_pages * page_size * 4 bytes of scratch, so max_pages should be no
+ * more than the longest sequence needs (a narrower view of the same table will do).
  * The library keeps 8 MB of workspace for each of up to 16 streams that have made a call
  * (further ones take over what is idle, or bring their own for the call), and the scratch
- * of key_weights in a stream-ordered pool; captured calls use the graph's memory.
+ * of key_weights in a stream-ordered pool that holds on to 512 MB at most, the workspaces
+ * included; captured calls use the graph's memory.
  * Calls on different streams, replays of different graphs and calls of different threads
  * may overlap. */
 int clove_paged_attention(const void* Q, long long q_stride, const clove_paged_cache* cache,

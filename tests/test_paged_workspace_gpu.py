@@ -196,3 +196,29 @@ def test_workspaces_of_gone_streams_are_taken_over(cuda):
     """Hundreds of streams, one after the other: what is kept stays bounded (16 workspaces of
     8 MB, and the pool's granularity), and results right; so with 40 in use at once."""
     _run(_STREAMS, "streams ok")
+
+
+_SCRATCH = r"""
+wide = torch.zeros((64, 1 << 14), dtype=torch.int32, device="cuda")
+wide[:, :2] = torch.arange(128, dtype=torch.int32, device="cuda").view(64, 2)
+lens = torch.full((64,), 20, dtype=torch.int32, device="cuda")
+q = torch.randn((64, 32, 128), device="cuda", generator=g).half()
+w, w2 = torch.zeros((400, 2, 16), device="cuda"), torch.zeros((400, 2, 16), device="cuda")
+want = cc.paged_attention(q, c, wide[:, :2], lens, key_weights=w2)
+torch.cuda.synchronize()
+free0 = torch.cuda.mem_get_info()[0]
+got = cc.paged_attention(q, c, wide, lens, key_weights=w)
+torch.cuda.synchronize()
+torch.cuda.synchronize()
+held = free0 - torch.cuda.mem_get_info()[0]
+print("held", held >> 20, "MB")
+assert torch.equal(got, want) and torch.equal(w, w2)
+assert held <= 512 << 20, held
+print("scratch ok")
+"""
+
+
+def test_large_scratch_goes_back(cuda):
+    """Key weights over wide page tables (2 GB of scratch): what the library's pool holds on
+    to afterwards is bounded."""
+    _run(_SCRATCH, "scratch ok")
