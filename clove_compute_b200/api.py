@@ -285,7 +285,8 @@ def debug_stream_k_plan(tiles: int, pairs: int, kb_total: int, force: int = 0) -
 
 
 def set_dispatch_override(path: int = 0, bn: int = 0, split: int = 0) -> None:
-    """Force a kernel family (tests): path 0 auto, 1 tensor core, 2 GEMV, 3 SIMT."""
+    """Force a kernel family (tests): path 0 auto, 1 tensor core, 2 GEMV, 3 SIMT.
+    qk_norm_rope goes by it too: 1 its streaming kernel, 2 its direct one, else auto."""
     check(lib().clove_set_dispatch_override(int(path), int(bn), int(split)))
 
 

@@ -294,7 +294,8 @@ int clove_debug_stream_k_plan(int tiles, int pairs, int kb_total, int force, int
  * bn: tensor-core N tile (0 = automatic; 32/64/128/256). split: cluster split-K
  * factor (0 = automatic, 1 = none, 2..8); with path 4 it selects the stream-K
  * schedule instead (0 automatic, 1 never, 2 whenever the tiles leave a partial
- * wave). Returns CLOVE_OK. */
+ * wave). clove_qk_norm_rope goes by path as well: 1 = its streaming kernel, 2 = its direct
+ * one, anything else = automatic (results are the same). Returns CLOVE_OK. */
 int clove_set_dispatch_override(int path, int bn, int split);
 
 /* Decode kernels (N <= 8 or M <= 8) start streaming their large operand -- the
