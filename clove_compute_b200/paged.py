@@ -106,6 +106,8 @@ def rope_table(length: int, rotary_dim: int, theta: float = 10000.0, device="cud
     are taken in 64 bits: in 32 the far positions would lose their fraction of a turn."""
     if length <= 0 or rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError("length must be positive, rotary_dim positive and even")
+    if not 0.0 < float(theta) < float("inf"):
+        raise ValueError("theta must be positive and finite")
     inv = float(theta) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device) / rotary_dim)
     a = torch.arange(length, dtype=torch.float64, device=device)[:, None] * inv[None, :]
     return torch.cat([a.cos(), a.sin()], 1).to(torch.float32)

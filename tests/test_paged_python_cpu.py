@@ -64,3 +64,10 @@ def test_torchs_own_refusals_are_passed_on():
         for wrong in ("text", None, 3, [1.0]):
             with pytest.raises(TypeError, match="Q must be a torch.Tensor"):
                 call(wrong)
+
+
+@pytest.mark.parametrize("theta", [0.0, -1.0, float("nan"), float("inf")])
+def test_rotation_base_out_of_range(theta):
+    """A base that is not positive and finite gives NaN angles."""
+    with pytest.raises(ValueError):
+        cc.rope_table(4, 64, theta, device="cpu")
