@@ -16,7 +16,7 @@
 //
 // Measured on one B200: 131071 keys, 8 heads, to 16001 (e4m3) 40 us: selection 26 (8 CTAs a
 // row: 7 to read the weights, the rest issue and barriers), copy 13. 8 sequences of up to
-// 32768 keys, 8 heads, to 8192 (fp16) 82 us: selection 25, copy 54 (0.95 of the copy rate).
+// 32768 keys, 8 heads, to 8192 (fp16) 82 us: selection 25, copy 54 (300 MB: 0.85 of the copy rate).
 // 4096 keys, 8 heads, to 1024: 15 us. Instructions that run once are fetched at about 0.3 us
 // per KB, so loops are kept short rather than unrolled.
 #include <algorithm>
@@ -435,8 +435,10 @@ int launch_evict_cache(const kern::EvictParams& p, const DeviceInfo& dev, cudaSt
     if (rc) return rc;
     g_evict_attr.fetch_or(bit, std::memory_order_acq_rel);
   }
-  // CTAs per (sequence, head): up to 8 while all of them fit on the GPU at once (one per
-  // SM) and each has 4096 keys, four per thread. (Clusters of 16 do not all fit: 131071 keys
+  // CTAs per (sequence, head): up to 8, doubled while all of them fit on the GPU at once (one
+  // per SM) and the table names more than 4096 keys, four per thread, for each of the present
+  // ones: a CTA of a cluster then has over 2048 keys of the table's width, of a row that is
+  // shorter than its table as many fewer. (Clusters of 16 do not all fit: 131071 keys
   // of 8 heads take 56 us with them, 42 us with 8. Twice as many CTAs as SMs: 8 sequences of
   // 32768 keys, 8 heads, ragged 82 -> 76 us, but of equal lengths 125 -> 134 us.)
   const long long rows = static_cast<long long>(p.batch) * p.cache.kv_heads;

@@ -8,7 +8,8 @@
 // element), so the kernel is bound by reading the cache once, and everything serves that:
 //
 // * Work split. An item is one (sequence, key head, block of up to 8 or 16 of its query
-//   heads); its keys are cut into tiles of 64. All tiles of all items, in order, are dealt
+//   heads); its keys are cut into tiles of 64, or of 128 where a row has 128 bytes or less
+//   (head_dim 64, and head_dim 128 in e4m3). All tiles of all items, in order, are dealt
 //   out evenly: CTA c of W takes tiles [c N / W, (c+1) N / W). So ragged batches, a single
 //   long sequence and many short ones all load every SM alike, with at most two unfinished
 //   items per CTA. Those are left as partial sums in a workspace; the CTA that finishes an
@@ -16,9 +17,11 @@
 //   Which CTA that is, a wrapping counter says, which is zero again when the item is done.
 //   (A second kernel for the join cost 3 us more per call.) Lengths are read on the device:
 //   one captured launch serves every step.
-// * Loads. Four warps per CTA, each with its own ring of 16-key K and V chunks filled by
-//   16-byte cp.async (any page size, order and strides), no CTA barrier until an item
-//   ends. Two CTAs per SM keep about 128 KB in flight per SM. The ring runs across items.
+// * Loads. Four warps per CTA, each with its own ring of K and V chunks of 16 keys (32 where
+//   tiles have 128) filled by 16-byte cp.async (any page size, order and strides), no CTA
+//   barrier until an item ends. Two CTAs per SM keep about 128 KB in flight per SM; for
+//   head_dim 256 only one fits, with 128 KB in 16 bits but 64 KB in e4m3. The ring runs
+//   across items.
 // * Products. S^T = K Q^T and O^T = V^T P^T as m16n8k16 matrix instructions with the keys
 //   (or head elements) as the 16 rows and 8 query heads as the columns: a group of up to 8
 //   heads wastes nothing that costs time. (tcgen05 wants 64 or 128 rows of queries.)
@@ -32,8 +35,8 @@
 //   only when some lane's score exceeds it.
 //
 // Measured, back to back on one B200: 64 sequences of up to 16384 keys, 32 / 8 heads of 128,
-// fp16 162 us (6.4 TB/s, 0.97 of the copy rate); 2 x 131071 keys, 64 / 8 heads, e4m3 103 us
-// (0.79; rows of 128 bytes at strides of 1 KB; 96 us with a head's rows side by side); 1 x
+// fp16 160 to 167 us (6.2 to 6.4 TB/s, 0.94 to 0.98 of the copy rate); 2 x 131071 keys, 64 / 8
+// heads, e4m3 102 to 109 us (0.75 to 0.80; rows of 128 bytes at strides of 1 KB; 96 us with a head's rows side by side); 1 x
 // 4096 keys, 32 / 32 heads, fp16 19 us, of which 9 read the cache, 4 pass before the first
 // key (length, page and key, three DRAM latencies in a row) and 4 in merging and joining.
 #pragma once
@@ -60,8 +63,10 @@ struct PagedShape {
   static constexpr int M = ROWB <= 128 ? 2 : 1;
   static constexpr int TILE = kPagedWarps * 16 * M;  // keys per CTA step
   static constexpr int CHUNK = 16 * M * ROWB;        // bytes of a warp's K (or V) chunk
-  // 24 KB of ring per warp where that holds three chunks (two CTAs per SM), else three
-  // chunks (head_dim 256 in 16 bits: one CTA per SM).
+  // 24 KB of ring per warp where that holds three chunks, else three chunks (head_dim 256 in
+  // 16 bits). Two CTAs fit on an SM but for head_dim 256, whose merge buffer takes 33 KB
+  // beside the rings: in e4m3 as well one CTA of 129 KB runs alone there (2 x 65536 keys, 32 /
+  // 8 heads: 114 us, 0.72 of the copy rate).
   static constexpr int STAGES = 24576 / (2 * CHUNK) >= 8 ? 8
                                 : 24576 / (2 * CHUNK) >= 3 ? 24576 / (2 * CHUNK) : 3;
   static constexpr int RING = STAGES * 2 * CHUNK;  // per warp

@@ -46,7 +46,7 @@ struct RopeParams {
 };
 
 // paged_attention_sm100.cuh
-constexpr int kPagedTile = 64;  // keys per CTA step, at least
+constexpr int kPagedTile = 64;  // keys per CTA step, at least (64 or 128)
 constexpr int kPagedCounters = 1 << 18;
 struct PagedAttnParams {
   const void* q;
@@ -64,7 +64,8 @@ struct PagedAttnParams {
   float scale_log2;  // scale * k_scale * log2(e)
   float v_scale;
   // Workspace: per CTA two partial results (heads in a block x D sums, maxima, totals) and
-  // one counter, zero before and after the call.
+  // one counter, zero before and after the call. Calls that run one after the other may
+  // share them.
   float* part_o;
   float* part_m;
   float* part_l;

@@ -143,7 +143,8 @@ def paged_attention(Q, cache: PagedCache, page_table, seq_lens, scale: float | N
     [pages, kv_heads, page_size] fp32, if given, gets the softmax weight of every attended
     key, summed over its query heads (added with accumulate=True); no page may then be in
     two sequences; and it takes 4 bytes of scratch per sequence, head and token that
-    page_table can name (page_table[:, :n] will do). scale defaults to 1/sqrt(D). An empty sequence gives zeros and -inf."""
+    page_table can name (page_table[:, :n] will do). scale defaults to 1/sqrt(D). An empty
+    sequence gives zeros and -inf; an infinite value in V gives NaN in its column."""
     fn = (_fast or _load()).paged_attention
     if stream is None:
         r = fn(Q, cache, page_table, seq_lens, scale, window, lse, key_weights, accumulate, O, None)

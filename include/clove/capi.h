@@ -191,8 +191,10 @@ typedef struct {
  * token t at t * *_stride elements (multiples of 8: column blocks of a fused projection).
  * y = x / sqrt(mean(x^2) + eps) * weight per head, weights [D] of the same type (both
  * NULL: no norm); then pair (i, i + rotary_dim/2), or (2i, 2i + 1) when interleaved, of
- * the first rotary_dim (a multiple of 16) elements is turned by row positions[t] of rope_table [table_len,
- * rotary_dim] fp32: rotary_dim/2 cosines, then as many sines. fp32, rounded once.
+ * the first rotary_dim (a multiple of 16) elements is turned by row positions[t] of
+ * rope_table [table_len, rotary_dim] fp32: rotary_dim/2 cosines, then as many sines. All of
+ * it in fp32, the sum of squares too (a bf16 row whose squares add up to more than fp32
+ * holds comes out as zeros), rounded once; an e4m3 cache saturates at +-448 and keeps NaN.
  * Q_out (may be Q with the same stride) gets the queries, K_out (may be K, or NULL with a
  * cache) the keys; with a cache, K and V rows also go to slot slots[t] (a negative slot:
  * not stored; distinct slots otherwise). A token with a negative position is padding:
@@ -213,7 +215,9 @@ int clove_qk_norm_rope(const void* Q, const void* K, const void* V, long long q_
  * apart; seq_lens [batch] counts the keys to attend to, the new token's among them. window
  * > 0: only the last `window` keys (pages before them are not looked up). lse (may be
  * NULL) [batch, num_heads]: log-sum-exp of the scaled scores. A length of 0 gives zeros
- * and -inf. A length outside [0, max_pages * page_size] is clamped and reported; a page
+ * and -inf. V is expected to be finite: an infinity among the attended values makes its
+ * column of the output NaN, whatever its sign (weights are multiplied in two halves, one of
+ * which may be zero or negative). A length outside [0, max_pages * page_size] is clamped and reported; a page
  * outside the cache reads as zeros and is reported (device error 3).
  * key_weights (may be NULL) [num_pages, num_kv_heads, page_size] fp32: each attended key's
  * softmax weight, summed over its query heads, is written there, or added when accumulate
