@@ -106,3 +106,28 @@ def test_attention_bf16_queries_of_wide_range(clove_lib, cuda, D, G, small):
             err, tol = (O[i].double() - o).abs(), b_o + ref.half_step(o.abs() + b_o, BF16)
             assert torch.all(err <= tol), (top, i, float((err / tol).max()))
             assert torch.all((lse[i].double() - l).abs() <= b_l), (top, i, float(((lse[i].double() - l).abs() / b_l).max()))
+
+
+@pytest.mark.parametrize("B,Hkv,cache_dtype", [(70001, 2, F16), (66000, 1, E4M3)])
+def test_attention_and_weights_of_huge_batches(clove_lib, cuda, B, Hkv, cache_dtype):
+    """More sequences than a grid dimension has blocks, of no, one or two keys: exact where the
+    answer is one value, half of two equal ones, and the weights of every key."""
+    D, G = 64, 2
+    g = torch.Generator(device="cuda").manual_seed(B)
+    V = torch.randint(-8, 9, (B, 2, Hkv, D), device="cuda", generator=g).to(cache_dtype)
+    cache = clove_lib.PagedCache(torch.zeros_like(V), V)
+    table = torch.randperm(B, device="cuda", generator=g).to(torch.int32)[:, None]
+    lens = (torch.arange(B, device="cuda") % 3).to(torch.int32)
+    w = torch.full((B, Hkv, 2), 7.0, device="cuda")
+    Q = torch.randn((B, Hkv * G, D), device="cuda", generator=g).to(F16)
+    O = clove_lib.paged_attention(Q, cache, table, lens, key_weights=w)
+    torch.cuda.synchronize()
+    assert clove_lib.device_error() == 0
+    v = V.float()[table[:, 0].long()]
+    want = torch.where((lens == 0)[:, None, None], 0.0, torch.where((lens == 1)[:, None, None], v[:, 0], v.mean(1)))
+    assert torch.equal(O.float(), want.repeat_interleave(G, 1))
+    seen = w[table[:, 0].long()]
+    n = lens[:, None].expand(-1, Hkv)
+    for t in (0, 1):
+        got = seen[:, :, t]
+        assert torch.all(got[n <= t] == 7.0) and torch.all((got[n > t] - G / n[n > t]).abs() <= 2.0 ** -21)

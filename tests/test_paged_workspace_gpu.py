@@ -112,7 +112,7 @@ def test_streams_forked_in_one_capture(cuda):
 
 _CAPTURE_BESIDE_EAGER = r"""
 import sys, threading
-cold = sys.argv[1] == "cold"
+cold, default = sys.argv[1] != "warm", sys.argv[1] == "default"
 O = torch.empty_like(Q)
 w = torch.zeros((400, 2, 16), device="cuda")
 mine, theirs = torch.cuda.Stream(), torch.cuda.Stream()
@@ -120,14 +120,24 @@ want = None
 if not cold:
     want = cc.paged_attention(Q, c, table, sl)
 x = torch.zeros(1 << 20, device="cuda")
+rope = cc.rope_table(4000, 128)
+spare, w2 = cc.PagedCache(K.clone(), V.clone()), torch.zeros((400, 2, 16), device="cuda")
+small, fresh = (torch.tensor([[a], [a + 1]], dtype=torch.int32, device="cuda") for a in (0, 2))
+few = torch.tensor([9, 3], dtype=torch.int32, device="cuda")
+k2 = Q[:, :2].contiguous()
+qo, ko = torch.empty_like(Q), torch.empty_like(k2)
+with torch.cuda.stream(theirs):  # (room for torch's allocator, which may not ask for more beside a capture)
+    room = torch.empty(1000, device="cuda")
 torch.cuda.synchronize()
 bad = []
 def eager():
     try:
         torch.cuda.set_device(0)
-        for s in (theirs, theirs):
-            cc.paged_attention(Q, c, table, sl, O=O, stream=s.cuda_stream)
-            cc.paged_attention(Q, c, table, sl, O=O, key_weights=w, stream=s.cuda_stream)
+        for s in (None, None) if default else (theirs.cuda_stream, theirs.cuda_stream):
+            cc.paged_attention(Q, c, table, sl, O=O, stream=s)
+            cc.paged_attention(Q, c, table, sl, O=O, key_weights=w, stream=s)
+            cc.qk_norm_rope(Q, k2, rope, sl, Q_out=qo, K_out=ko, stream=s)
+            cc.evict_cache(spare, w2, small, few, fresh, 4, 1, stream=s)
     except Exception as e:
         bad.append(e)
 gr = torch.cuda.CUDAGraph()
@@ -148,10 +158,10 @@ print("beside ok")
 """
 
 
-@pytest.mark.parametrize("start", ["cold", "warm"])
+@pytest.mark.parametrize("start", ["cold", "warm", "default"])
 def test_eager_calls_while_another_thread_captures(cuda, start):
-    """The eager calls of one thread, the process's first ones too, and a capture under way in
-    another do not disturb each other."""
+    """The eager calls of one thread, the process's first ones too, on the default stream or
+    another, and a capture under way in another thread do not disturb each other."""
     r = subprocess.run([sys.executable, "-c", _SETUP + _CAPTURE_BESIDE_EAGER, start], cwd=ROOT, capture_output=True,
                        text=True, timeout=600)
     assert r.returncode == 0 and "beside ok" in r.stdout, (r.stdout[-500:], r.stderr[-2500:])
