@@ -436,9 +436,8 @@ int launch_evict_cache(const kern::EvictParams& p, const DeviceInfo& dev, cudaSt
     g_evict_attr.fetch_or(bit, std::memory_order_acq_rel);
   }
   // CTAs per (sequence, head): up to 8, doubled while all of them fit on the GPU at once (one
-  // per SM) and the table names more than 4096 keys, four per thread, for each of the present
-  // ones: a CTA of a cluster then has over 2048 keys of the table's width, of a row that is
-  // shorter than its table as many fewer. (Clusters of 16 do not all fit: 131071 keys
+  // per SM) and each has more than 4096 keys, four per thread; after the doubling it has more
+  // than 2048. That goes by the table's width: shorter rows leave their CTAs less. (Clusters of 16 do not all fit: 131071 keys
   // of 8 heads take 56 us with them, 42 us with 8. Twice as many CTAs as SMs: 8 sequences of
   // 32768 keys, 8 heads, ragged 82 -> 76 us, but of equal lengths 125 -> 134 us.)
   const long long rows = static_cast<long long>(p.batch) * p.cache.kv_heads;
