@@ -119,5 +119,6 @@ def fastcall():
     try:
         from . import _fastcall
     except ImportError as e:
-        raise ImportError("_fastcall is missing for this Python version: build it with `python -m clove_compute_b200.build`") from e
+        raise ImportError("_fastcall is missing for this Python version: build it with "
+                          "`python -m clove_compute_b200.build`") from e
     return _fastcall

@@ -37,8 +37,9 @@
 // Measured, back to back on one B200: 64 sequences of up to 16384 keys, 32 / 8 heads of 128,
 // fp16 160 to 167 us (6.2 to 6.4 TB/s, 0.94 to 0.98 of the copy rate); 2 x 131071 keys, 64 / 8
 // heads, e4m3 102 to 109 us (0.75 to 0.80; rows of 128 bytes at strides of 1 KB; 96 us with a
-// head's rows side by side); 1 x 4096 keys, 32 / 32 heads, fp16 19 us, of which 9 read the cache, 4 pass before the first
-// key (length, page and key, three DRAM latencies in a row) and 4 in merging and joining.
+// head's rows side by side); 1 x 4096 keys, 32 / 32 heads, fp16 19 us, of which 9 read the
+// cache, 4 pass before the first key (length, page and key, three DRAM latencies in a row)
+// and 4 in merging and joining.
 #pragma once
 
 #include <cuda_runtime.h>
